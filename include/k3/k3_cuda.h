@@ -43,6 +43,9 @@ enum {
     K3D_ETIMEOUT = 9       /* a bounded device-side wait gave up */
 };
 
+/* Element types (checkpoint tensors, and operators that take more than one). */
+enum { K3D_DT_U8 = 1, K3D_DT_BF16 = 2, K3D_DT_F16 = 3, K3D_DT_F32 = 4 };
+
 /* Select the CUDA device and create the library stream. Idempotent for the same
  * device; the k3.h entry points call k3d_init(0) on first use if nobody did. One device
  * per process: once the context exists, k3d_init with another device returns K3D_EINVAL
@@ -431,6 +434,109 @@ int    k3d_moe_swiglu_a2a_dev(float *out, const float *x, const K3dMoeW *w, cons
 int    k3d_a2a_plan(const int *idx, int TK, int n_experts, int nranks, int *cnt, int *off,
                     int *pos);
 
+/* ------------------------------------------------ serving: pages, 4-bit cache ---- */
+/* Operators of a serving loop whose requests have lengths of their own and bring one or
+ * several new tokens a step (a prompt, a token, drafted tokens): pages planned on the device,
+ * the latent cache held in 4 bits, attention over it, and tokens drawn from the logits. No
+ * reference counterpart except where noted: the CPU engine holds one sequence in one
+ * contiguous fp32 cache and takes the argmax. As everywhere here: device pointers,
+ * asynchronous on the library stream, no allocation, capturable into a CUDA graph. */
+
+/* Page tables and slot maps of B requests (at most 8192) in one plan. Request b holds `len`
+ * positions and brings n_new[b] more (0 is allowed); after the call it holds exactly
+ * ceil((len[b] + n_new[b]) / page) pages: missing ones come off the free stack, surplus ones
+ * (drafts that were rejected, a request that ended: len 0 and n_new 0) go back onto it.
+ * Writes row_start[B + 1] (prefix sum of n_new), kv_len[B] = len + n_new, and for each new
+ * row its position pos and its slot = page id * page + position % page; the rows from
+ * row_start[B] to N get -1, so a step padded to N rows is safe. free_list[0 .. *n_free) are
+ * the free page ids, the top last. Pages given back leave -1 in the table and are pushed in
+ * descending (request, page) order, so taking pages and giving them back restores the stack.
+ * *status receives a K3D_PLAN_* code; with any but K3D_PLAN_OK table, held, free_list and
+ * n_free are unchanged, every row_start and kv_len is 0 and every pos and slot -1: a
+ * scheduler reads it when it next looks at the device. The arrays must not overlap. */
+enum {
+    K3D_PLAN_OK = 0,
+    K3D_PLAN_PAGES = 1,    /* the free stack is short */
+    K3D_PLAN_ROWS = 2,     /* more new rows than N */
+    K3D_PLAN_TABLE = 3,    /* a request needs more than max_pages pages */
+    K3D_PLAN_BAD = 4       /* negative or overflowing length, held or n_free out of range */
+};
+typedef struct {
+    int  page;             /* positions per page */
+    int  n_pages;          /* page ids are 0 .. n_pages - 1; n_pages * page below 2^31 */
+    int  max_pages;        /* columns of table */
+    int *table;            /* [B][max_pages] page ids, -1 where none is held */
+    int *held;             /* [B] pages held */
+    int *free_list;        /* [n_pages] */
+    int *n_free;           /* one int */
+} K3dPages;
+int    k3d_page_plan(const K3dPages *p, const int *len, const int *n_new, int B, int N,
+                     int *row_start, int *kv_len, int *pos, int *slots, int *status);
+
+/* The paged latent cache in 4 bits. A row (one position) is kv_lora normalised latent values
+ * and qk_rope rotated key values, as in the bf16 cache of k3d_mla_decode (1152 bytes at
+ * 512 + 64; here 417). It is held in units of 2^e with e the row's own exponent (one byte,
+ * e + 127): every 16 latent values share an E4M3 scale s = e4m3(max|x| 2^-e / 6) and are E2M1
+ * codes of x 2^-e / s, ties to even, the even element in the low nibble; the rotated key is
+ * fp16 of x 2^-e. e is the smallest integer >= -100 with max|latent| <= 2688 2^e and
+ * max|rope| <= 32768 2^e. A row that holds a NaN or an infinity is NaN throughout (exponent
+ * byte 255). A page holds `page` rows as four arrays one after the other: codes
+ * [page][kv_lora/2], scales [page][kv_lora/16], rope [page][qk_rope] fp16, exponent bytes
+ * [page]; page ids index the pool, which is 16-byte aligned. */
+typedef struct {
+    int kv_lora;           /* a multiple of 128 up to 512 */
+    int qk_rope;           /* a multiple of 16 up to 64; 0: none */
+    int page;              /* a multiple of 16 up to 1024 */
+    int n_pages;           /* n_pages * page below 2^31 */
+} K3dCache4;
+/* Bytes of the whole pool (0 for a shape that is not supported). */
+size_t k3d_cache4_bytes(const K3dCache4 *c);
+/* Quantises N rows of x (dtype K3D_DT_F32 or K3D_DT_BF16, ldx elements apart) into their
+ * slots, and reads the rows of `slots` back as fp32 or bf16. A slot of -1 is passed over (the
+ * row of the destination is left as it was); any other slot outside the pool raises the
+ * device error K3D_EBOUND and is passed over. The slots of one store must differ: of two
+ * rows with the same slot neither is stored whole. */
+int    k3d_cache4_store(const K3dCache4 *c, void *pool, const void *x, int dtype, size_t ldx,
+                        const int *slots, int N);
+int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtype, size_t ldo,
+                       const int *slots, int N);
+/* Absorbed MLA attention over the paged 4-bit cache (the attention step of k3d_mla_decode,
+ * following k3_mla_cached, k3_ops.c:321-410): q [N][H][kv_lora + qk_rope] are the absorbed
+ * queries of the new rows, out [N][H][kv_lora] the attended latents, each fp32 or bf16 and
+ * 16-byte aligned. Request b owns the rows row_start[b] .. row_start[b + 1] and kv_len[b]
+ * cached positions, its new ones (stored before this call) among them; its row j sees the
+ * first kv_len[b] - rows + j + 1 positions, and gets zeros when that is none. Rows from
+ * row_start[B] to N are left as they were. table [B][max_pages] as in K3dPages. Scores,
+ * softmax and sums are fp32; q is rounded to fp16 in units of its row (exact for bf16) and
+ * the softmax weights to fp16. A page id outside the pool, a kv_len above max_pages * page,
+ * or a row_start that is not a prefix sum within N raises K3D_EBOUND; such positions count as
+ * not there. The workspace belongs to the call until it has run: two calls that may run at
+ * the same time (two streams, two graphs) need one each. */
+size_t k3d_mla_attend4_ws_bytes(const K3dCache4 *c, int B, int N, int H);
+int    k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const K3dCache4 *c,
+                       const void *pool, const int *table, int max_pages, const int *row_start,
+                       const int *kv_len, int B, int N, int H, float scale, void *ws,
+                       size_t ws_bytes);
+/* p[r] = softmax(logits[r] / temp[r]) over rows of vocab; temp NULL is 1, and a temperature
+ * that is not above 0 puts 1 on the first maximum, as k3d_lm_head_argmax picks it. A NaN logit
+ * counts as minus infinity; places at +inf share the whole; a row with nothing above minus
+ * infinity is zeros. p may be logits itself (in place). */
+int    k3d_logits_softmax(float *p, const float *logits, const float *temp, int rows, int vocab);
+/* Verification of up to K drafted tokens per request (K at most 32; n_draft[b] of them, NULL:
+ * K) against the target's probabilities target [B][K + 1][vocab], row i of a request being
+ * the distribution at draft i's place. draft [B][K][vocab] are the probabilities the drafts
+ * ids [B][K] were drawn from, NULL: each was certain. Draft i is kept while
+ * u_accept[b][i] q_i(d) < p_i(d); n_accept[b] of them are. Then one more token is drawn at
+ * u_sample[b] (in [0, 1)) of the running sum of max(p - q, 0) at the first rejected place, or
+ * of p behind the last draft; each weight counts in whole 2^-44 (truncated, at most 1, NaN 0),
+ * so that the result does not depend on the order of the sum. Where max(p - q, 0) is nothing
+ * anywhere the draw is from p. tokens [B][K + 1] receives the kept drafts, the drawn token (-1
+ * where p holds nothing either) and -1 behind it. A draft id outside the vocabulary is never
+ * kept. */
+int    k3d_spec_verify(int *tokens, int *n_accept, const float *target, const float *draft,
+                       const int *ids, const int *n_draft, const float *u_accept,
+                       const float *u_sample, int B, int K, int vocab);
+
 /* ----------------------------------------------------------- decode stack ---- */
 typedef struct {
     int   hidden, vocab, n_layers;
@@ -518,7 +624,6 @@ int       k3d_model_state_load(K3dModel *m, const char *path, int *seq, int seq_
  * element size, inside the file); lookups are O(1). Host only: none of the k3d_ckpt_*
  * calls touches the GPU. k3d_ckpt_error gives the reason of the last failure. */
 typedef struct K3dCkpt K3dCkpt;
-enum { K3D_DT_U8 = 1, K3D_DT_BF16 = 2, K3D_DT_F16 = 3, K3D_DT_F32 = 4 };
 typedef struct {
     int     shard, dtype, ndim;
     int64_t shape[4];

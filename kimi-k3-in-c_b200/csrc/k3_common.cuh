@@ -273,5 +273,5 @@ __device__ __forceinline__ float silu_f(float g) { return g / (1.0f + expf(-g));
 enum {
     K3_SITE_MXFP4 = 1, K3_SITE_ROUTER = 2, K3_SITE_MOE = 3, K3_SITE_GEMV = 4,
     K3_SITE_KDA = 5, K3_SITE_MLA = 6, K3_SITE_SMALL = 7, K3_SITE_STACK = 8,
-    K3_SITE_EP = 9
+    K3_SITE_EP = 9, K3_SITE_CACHE4 = 10
 };

@@ -17,6 +17,9 @@ K3D_OK = 0
 K3D_ENODEV, K3D_EINVAL, K3D_ENOMEM, K3D_ECUDA, K3D_EDEVICE = 1, 2, 3, 4, 5
 K3D_EUNSUPPORTED, K3D_ENCCL, K3D_EBOUND, K3D_ETIMEOUT = 6, 7, 8, 9
 
+K3D_DT_U8, K3D_DT_BF16, K3D_DT_F16, K3D_DT_F32 = 1, 2, 3, 4
+K3D_PLAN_OK, K3D_PLAN_PAGES, K3D_PLAN_ROWS, K3D_PLAN_TABLE, K3D_PLAN_BAD = 0, 1, 2, 3, 4
+
 vp = C.c_void_p
 i32 = C.c_int
 f32 = C.c_float
@@ -108,6 +111,15 @@ class K3dStateInfo(C.Structure):
 class K3dCkptTensor(C.Structure):
     _fields_ = [("shard", i32), ("dtype", i32), ("ndim", i32), ("shape", C.c_int64 * 4),
                 ("off", C.c_int64), ("nbytes", C.c_int64)]
+
+
+class K3dPages(C.Structure):
+    _fields_ = [("page", i32), ("n_pages", i32), ("max_pages", i32), ("table", vp), ("held", vp),
+                ("free_list", vp), ("n_free", vp)]
+
+
+class K3dCache4(C.Structure):
+    _fields_ = [("kv_lora", i32), ("qk_rope", i32), ("page", i32), ("n_pages", i32)]
 
 
 class K3dStackCfg(C.Structure):
@@ -266,6 +278,16 @@ _PROTOS = {
     "k3d_moe_swiglu_a2a": (i32, [vp, vp, C.POINTER(K3dMoeW), C.POINTER(K3dMoeShape), i32, i32, i32, vp,
                                  vp, vp, sz]),
     "k3d_a2a_plan": (i32, [vp, i32, i32, i32, vp, vp, vp]),
+    # serving
+    "k3d_page_plan": (i32, [C.POINTER(K3dPages), vp, vp, i32, i32, vp, vp, vp, vp, vp]),
+    "k3d_cache4_bytes": (sz, [C.POINTER(K3dCache4)]),
+    "k3d_cache4_store": (i32, [C.POINTER(K3dCache4), vp, vp, i32, sz, vp, i32]),
+    "k3d_cache4_load": (i32, [C.POINTER(K3dCache4), vp, vp, i32, sz, vp, i32]),
+    "k3d_mla_attend4_ws_bytes": (sz, [C.POINTER(K3dCache4), i32, i32, i32]),
+    "k3d_mla_attend4": (i32, [vp, i32, vp, i32, C.POINTER(K3dCache4), vp, vp, i32, vp, vp, i32, i32, i32,
+                              f32, vp, sz]),
+    "k3d_logits_softmax": (i32, [vp, vp, vp, i32, i32]),
+    "k3d_spec_verify": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32]),
     # stack
     "k3d_model_create": (vp, [C.POINTER(K3dStackCfg), u64]),
     "k3d_model_destroy": (None, [vp]),
