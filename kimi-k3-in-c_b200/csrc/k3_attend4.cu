@@ -6,13 +6,50 @@
 //   o[r]    = sum_t softmax(s[r])[t] row[t][0 .. kv)
 // Row r = (new token j of request b, head): it sees the first kv_len[b] - new_b + j + 1
 // positions (none: zeros).
+//
+// WORK. The rows of a request are contiguous in q ([N][H] flattened); an item is up to 64 of
+// them (whole tokens when H <= 64, else 64 heads of one token) and a unit is one item times
+// one tile of 64 positions. The units of all items, item-major, are cut into one contiguous
+// range per CTA, so ragged lengths balance themselves. An item that one CTA covers is written
+// directly; the parts of a cut item (at most two per CTA) go to the workspace as
+// (unnormalised o, max, sum) and a second kernel adds them in CTA order.
+//
+// PRODUCTS (tcgen05, fp16 x fp16, fp32 accumulators in tensor memory). A tile's rows are
+// widened once to fp16 in units of 2^e (exact, k3_cache4.cuh), 64 values to a 128-byte
+// swizzled panel row, and serve both products from the same bytes:
+//   S [64 rows][64 keys]     = Q K^T      M = 64, K-major A = Q and B = the tile
+//   O^T [kv][rows] (4 x 128) += V^T P^T   M = 128 latents, A = the tile read MN-major,
+//                                         B = P, K-major, N = the rows rounded up to 16
+// O^T rather than O keeps the accumulator of 64 rows in 256 of the 512 columns, which leaves
+// room for two S; O of 64 rows and 512 latents would fill all of them. q is fp16 in units of
+// its row (exact for bf16 within 2^-29 of the row's largest value). The softmax works on
+// a = s log2(e) + e: P = 2^(a - m), rounded to fp16 (2^-12 on average, an eighth of the step
+// of a bf16 result), carries the key's unit 2^e, while the sum takes 2^(s - m) in fp32. m is
+// a reference that moves only when a tile's maximum passes it by 2^8, so that the
+// accumulator is rescaled rarely; P is kept below 2^15 and weights down to 2^-31 of the
+// largest keep their value.
+//
+// ROLES (416 threads): warps 0-7 load a tile ahead into registers, widen and store it;
+// warps 8-11 do the softmax, the rescaling and the results; warp 12 issues the MMAs, in the
+// order S(t + 1), O(t). All 12 load Q. Every wait is bounded (k3_bulk.cuh).
+#include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"
 
 namespace k3 {
-namespace {
+namespace at4 {
 
-struct Attend {
+using namespace bulk;
+
+constexpr int kT = 64;                    // positions per tile
+constexpr int kR = 64;                    // rows per item
+constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
+constexpr int kThreads = 416;
+constexpr int kMaxUnits = 1 << 30;
+constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
+constexpr float kStep = 8.f;              // m moves when a tile passes it by this
+
+struct Args {
     Pool4 d;
     const void *q;
     void *out;
@@ -20,103 +57,853 @@ struct Attend {
     int max_pages, B, N, H;
     int q_f32, out_f32;
     float scale;
+    float *part;                          // [grid][2][64][kv]
+    float2 *ml;                           // [grid][2][64] (max, sum), base 2
+    int4 *info;                           // [grid][2]: {u0, item begin, item end, 0}, {row0, rows, 0, 0}
 };
 
-// The request of token n, or -1 behind the last row.
-__device__ __forceinline__ int request_of_row(const int *start, int B, int n)
+struct Smem {                             // offsets from the 1024-byte aligned base
+    uint32_t q, k, p, kinfo, row, bars, total;
+};
+
+__host__ __device__ inline Smem smem_layout(int kv, int rope)
 {
-    if (n >= start[B]) return -1;
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (start[mid] <= n) lo = mid; else hi = mid;
-    }
-    return lo;
+    Smem s;
+    const uint32_t panels = kv / 64 + (rope ? 1 : 0);
+    s.q = 0;
+    s.k = s.q + panels * kPanel;
+    s.p = s.k + 2 * panels * kPanel;
+    s.kinfo = s.p + kR * 128;             // float [2][64]: e of each position
+    s.row = s.kinfo + 2 * kT * 4;         // float [64] score factor, int [64] limit, float [64] x 2
+    s.bars = s.row + 4 * kR * 4;
+    s.total = s.bars + 160;
+    return s;
 }
 
-// grid (N, ceil(H / 8)), one warp per head, tiles of 16 positions as fp32 in shared memory.
-__global__ void __launch_bounds__(256) k_attend4_plain(Attend a)
+// One request as the scheduler sees it.
+struct Req {
+    int n, kvl, items, tiles;
+};
+
+__device__ __forceinline__ Req request(const Args &a, int b)
 {
+    Req r;
+    const int r0 = a.row_start[b], r1 = a.row_start[b + 1];
+    int n = r1 - r0, kvl = a.kv_len[b];
+    const int cap = a.max_pages * a.d.page;
+    if (r0 < 0 || n < 0 || r1 > a.N || kvl < 0 || kvl > cap) {
+        k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, r1, kvl);
+        if (r0 < 0 || n < 0 || r1 > a.N) n = 0;
+        kvl = max(0, min(kvl, cap));
+    }
+    r.n = n;
+    r.kvl = kvl;
+    const int per = a.H <= kR ? kR / a.H : 1;
+    r.items = a.H <= kR ? (n + per - 1) / per : n * ((a.H + kR - 1) / kR);
+    r.tiles = max(1, (kvl + kT - 1) / kT);
+    return r;
+}
+
+// The piece of an item that a CTA works on, and the rows of it.
+struct Seg {
+    int b, n, kvl;
+    int row0, rows;                       // flattened rows of q
+    int j0;                               // new token of the first row
+    int t0, t1;                           // tiles [t0, t1), cut to what the item sees
+    int begin, end;                       // units of the whole item
+    bool whole;
+};
+
+struct Cursor {
+    int u, u1, b, pre;
+    Req r;
+};
+
+__device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
+{
+    if (c.u >= c.u1) return false;
+    while (c.u >= c.pre + c.r.items * c.r.tiles) {
+        c.pre += c.r.items * c.r.tiles;
+        c.b++;
+        c.r = request(a, c.b);
+    }
+    const int item = (c.u - c.pre) / c.r.tiles;
+    s.b = c.b;
+    s.n = c.r.n;
+    s.kvl = c.r.kvl;
+    s.begin = c.pre + item * c.r.tiles;
+    s.end = s.begin + c.r.tiles;
+    const int first = a.row_start[c.b];
+    int last;
+    if (a.H <= kR) {
+        const int per = kR / a.H;
+        s.j0 = item * per;
+        const int tok = min(per, c.r.n - s.j0);
+        s.row0 = (first + s.j0) * a.H;
+        s.rows = tok * a.H;
+        last = s.j0 + tok - 1;
+    } else {
+        const int hc = (a.H + kR - 1) / kR;
+        s.j0 = last = item / hc;
+        const int h0 = (item % hc) * kR;
+        s.row0 = (first + s.j0) * a.H + h0;
+        s.rows = min(kR, a.H - h0);
+    }
+    const int stop = min(c.u1, s.end);
+    const int seen = max(0, c.r.kvl - c.r.n + last + 1);
+    s.t0 = c.u - s.begin;
+    s.t1 = min(stop - s.begin, (seen + kT - 1) / kT);
+    s.whole = c.u == s.begin && stop == s.end;
+    c.u = stop;
+    return true;
+}
+
+// ------------------------------------------------------------------- tcgen05 wrappers ----
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory"); }
+
+// SWIZZLE_128B descriptors: K-major (8-row groups 1024 B apart), and MN-major (64-element
+// blocks `lead` bytes apart, groups of 8 k 1024 B apart).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// kind::f16, fp32 D, fp16 A and B
+__device__ __forceinline__ uint32_t idesc(int M, int N, int a_mn)
+{
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum) : "memory");
+}
+
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+
+#define K3_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
+                    "=r"(r[i + 6]), "=r"(r[i + 7])
+
+// 16 lanes x 64 columns: element 4 i + 2 h + e is row lane / 4 + 8 h, column 8 i + 2 (lane % 4) + e
+__device__ __forceinline__ void ld_s(uint32_t taddr, float v[32])
+{
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+                 "%26,%27,%28,%29,%30,%31}, [%32];"
+                 : K3_R8(r, 0), K3_R8(r, 8), K3_R8(r, 16), K3_R8(r, 24) : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void ld16(uint32_t taddr, float v[16])
+{
+    uint32_t r[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : K3_R8(r, 0), K3_R8(r, 8) : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void st16(uint32_t taddr, const float v[16])
+{
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) r[i] = __float_as_uint(v[i]);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+                    "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+                    "r"(r[15]) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// 2^e of a whole e in [-126, 127] kept as a float: e + 127 lands in the low mantissa bits
+__device__ __forceinline__ float unit(float e)
+{
+    return __uint_as_float(__float_as_uint(e + 12583039.0f) << 23);
+}
+
+// Byte `at` of row `row` in a panel of 128-byte rows, 16-byte units swizzled by the row.
+__device__ __forceinline__ uint32_t swz(int row, int unit) { return (uint32_t)(row * 128 + ((unit ^ (row & 7)) << 4)); }
+
+// 16 bytes that no other thread reads, past L1 (a plain load: earlier work of the stream may
+// still have been writing the pool when this kernel was launched)
+__device__ __forceinline__ uint4 ld_v4(const void *p)
+{
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+    return r;
+}
+
+// ------------------------------------------------------------------------ the widening ----
+// Thread (position, part) of a tile: 16 bytes of codes and 2 scales of every 128 latents,
+// and up to two 16-byte units of the rope key.
+template <int NB>
+struct Raw {
+    uint4 code[NB];
+    uint32_t scale[NB];                   // two E4M3 bytes
+    uint4 rope[2];
+    int e;                                // exponent byte, or -1: not there
+};
+
+// The page of a position, or -1 where it is not there (past the length, or no page of the pool).
+__device__ __forceinline__ int page_at(const Args &a, int b, int pos, int kvl)
+{
+    if (pos >= kvl) return -1;
+    const int pg = a.table[(size_t)b * a.max_pages + pos / a.d.page];
+    if (pg < 0 || pg >= a.d.n_pages) {
+        k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, pg, pos);
+        return -1;
+    }
+    return pg;
+}
+
+template <int NB>
+__device__ __forceinline__ void load_raw(Raw<NB> &r, const Args &a, int pg, int pos, int part)
+{
+    r.e = -1;
+#pragma unroll
+    for (int i = 0; i < NB; i++) { r.code[i] = make_uint4(0u, 0u, 0u, 0u); r.scale[i] = 0u; }
+    r.rope[0] = r.rope[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (pg < 0) return;
+    const uint8_t *base = a.d.p + (size_t)pg * a.d.page_bytes;
+    const int in = pos % a.d.page;
+    const uint8_t *c = base + (size_t)in * (NB * 64) + part * 16;
+    const uint8_t *s = base + a.d.o_scale + in * (NB * 8) + part * 2;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        r.code[i] = ld_v4(c + i * 64);
+        r.scale[i] = *reinterpret_cast<const uint16_t *>(s + i * 8);
+    }
+    const uint8_t *rp = base + a.d.o_rope + (size_t)in * 2 * a.d.rope;
+    if (part < a.d.rope / 8) r.rope[0] = ld_v4(rp + part * 16);
+    if (part + 4 < a.d.rope / 8) r.rope[1] = ld_v4(rp + (part + 4) * 16);
+    r.e = base[a.d.o_exp + in];
+}
+
+// Widens one thread's share into the tile's panels. Of the four 16-byte units that a thread
+// writes per 128 latents, parts 2 and 3 take the second pair first: the eight threads of a
+// store phase (two positions x four parts) then hit eight different 16-byte banks.
+template <int NB>
+__device__ __forceinline__ void widen(const Raw<NB> &r, uint32_t tile, int row, int part, int rope)
+{
+    const bool swap = part & 2;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        uint32_t s2;                      // the two scales as f16x2
+        asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(s2) : "r"(r.scale[i]));
+        const uint32_t lo = __byte_perm(s2, s2, 0x1010), hi = __byte_perm(s2, s2, 0x3232);
+        const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
+        const uint32_t panel = tile + (uint32_t)(2 * i + (part >> 1)) * kPanel;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t word = swap ? w[j ^ 2] : w[j];
+            const uint32_t f = ((j & 2) != 0) != swap ? hi : lo;
+            uint32_t h[4];
+            e2m1x8_to_f16x8(word, h);
+            const int unit = (part & 1) * 4 + (swap ? j ^ 2 : j);
+            sts16(panel + swz(row, unit), make_uint4(hmul2(h[0], f), hmul2(h[1], f), hmul2(h[2], f), hmul2(h[3], f)));
+        }
+    }
+    const uint32_t panel = tile + (uint32_t)(2 * NB) * kPanel;
+    if (part < rope / 8) sts16(panel + swz(row, part), r.rope[0]);
+    if (part + 4 < rope / 8) sts16(panel + swz(row, part + 4), r.rope[1]);
+}
+
+// ------------------------------------------------------------------------------- Q ----
+// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the row's largest value in
+// [2^13, 2^14)), the score factor and the number of positions the row sees.
+__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
+{
+    const int W = a.d.kv + a.d.rope, chunks = W / 8;
+    for (int r = warp; r < kR; r += 12) {
+        if (r >= s.rows) {
+            if (lane == 0) { fac[r] = 0.f; lim[r] = 0; }
+            continue;
+        }
+        const size_t at = (size_t)(s.row0 + r) * W;
+        float v[3][8];
+#pragma unroll
+        for (int c = 0; c < 3; c++) {
+            const int ch = lane + 32 * c;
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[c][k] = 0.f;
+            if (ch < chunks) {
+                if (a.q_f32) {
+                    const float4 *p = reinterpret_cast<const float4 *>((const float *)a.q + at + ch * 8);
+                    const float4 x = p[0], y = p[1];
+                    v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
+                    v[c][4] = y.x; v[c][5] = y.y; v[c][6] = y.z; v[c][7] = y.w;
+                } else {
+                    const uint4 x = *reinterpret_cast<const uint4 *>((const uint16_t *)a.q + at + ch * 8);
+                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        v[c][2 * k] = __uint_as_float(u[k] << 16);
+                        v[c][2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                    }
+                }
+            }
+        }
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < 3; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[c][k]));
+        m = warp_max(m);
+        int e = 0;
+        if (m > 0.f && m <= 3.4028234e38f) {
+            frexpf(m, &e);
+            e = max(e, -110);
+        }
+        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+#pragma unroll
+        for (int c = 0; c < 3; c++) {
+            const int ch = lane + 32 * c;
+            if (ch < chunks) {
+                uint32_t h[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const __half2 t = __floats2half2_rn(v[c][2 * k] * up, v[c][2 * k + 1] * up);
+                    h[k] = *reinterpret_cast<const uint32_t *>(&t);
+                }
+                sts16(sq + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
+            }
+        }
+        if (lane == 0) {
+            // scale log2(e) 2^(e - 14), the power in two factors (e - 14 may be below -126)
+            const int k = e - 14, k1 = k >> 1;
+            fac[r] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
+                     __uint_as_float((uint32_t)(k - k1 + 127) << 23);
+            const int j = s.j0 + (a.H <= kR ? r / a.H : 0);
+            lim[r] = max(0, s.kvl - s.n + j + 1);
+        }
+    }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__ Args a)
+{
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ long long red[13];
+    __shared__ int s_cur[2];
+    const uint32_t raw = saddr(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char *gb = smem_raw + (base - raw);
+    const Smem L = smem_layout(NB * 128, a.d.rope);
+    const uint32_t panels = NB * 2 + (a.d.rope ? 1 : 0);
+    float *kinfo = reinterpret_cast<float *>(gb + L.kinfo);
+    float *fac = reinterpret_cast<float *>(gb + L.row);
+    int *lim = reinterpret_cast<int *>(gb + L.row + kR * 4);
+    float *rowf = reinterpret_cast<float *>(gb + L.row + 2 * kR * 4);   // rescale factors, then 1 / sum
+    int *flags = reinterpret_cast<int *>(gb + L.row + 3 * kR * 4);      // [2][4]
+    const uint32_t b_qfull = base + L.bars, b_qempty = b_qfull + 8;
+    const uint32_t b_kfull = b_qfull + 16, b_sfull = b_qfull + 32, b_pfull = b_qfull + 48, b_pv = b_qfull + 56;
+    const uint32_t b_drain = b_qfull + 72;
+    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 96);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 100);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        mbar_init(b_qfull, 12);
+        mbar_init(b_qempty, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(b_kfull + 8 * i, 8);
+            mbar_init(b_sfull + 8 * i, 1);
+            mbar_init(b_pv + 8 * i, 1);
+        }
+        mbar_init(b_pfull, 4);
+        mbar_init(b_drain, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(saddr(tslot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_before();
+    }
     pdl_wait();
     pdl_trigger();
-    __shared__ float tile[16][576 + 4];
-    const int n = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.y * 8 + warp;
-    const int W = a.d.kv + a.d.rope;
-    const int b = request_of_row(a.row_start, a.B, n);
-    if (b < 0) return;
-    const int j = n - a.row_start[b], nw = a.row_start[b + 1] - a.row_start[b];
-    int kvl = a.kv_len[b];
-    if (kvl > a.max_pages * a.d.page) {
-        if (threadIdx.x == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, kvl, 2);
-        kvl = a.max_pages * a.d.page;
+
+    // ---- this CTA's units: the requests' totals, then the request that holds the first unit
+    const int per = (a.B + kThreads - 1) / kThreads;
+    const int rb0 = min(a.B, tid * per), rb1 = min(a.B, rb0 + per);
+    long long mine = 0;
+    for (int b = rb0; b < rb1; b++) {
+        const Req r = request(a, b);
+        mine += (long long)r.items * r.tiles;
     }
-    const int seen = max(0, kvl - nw + j + 1);
-    float q[18], acc[18];
+    long long incl = mine;
 #pragma unroll
-    for (int i = 0; i < 18; i++) {
-        q[i] = acc[i] = 0.f;
-        const int c = lane + 32 * i;
-        if (h < a.H && c < W) {
-            const size_t at = ((size_t)n * a.H + h) * W + c;
-            q[i] = a.q_f32 ? ((const float *)a.q)[at] : bf16_to_f32(((const uint16_t *)a.q)[at]);
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) red[warp] = incl;
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = *tslot;
+    long long lead = incl - mine, total = 0;
+    for (int i = 0; i < 13; i++) {
+        if (i < warp) lead += red[i];
+        total += red[i];
+    }
+    if (total > kMaxUnits) {                              // unit numbers are 31-bit
+        if (tid == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, a.N, a.H, 4);
+        total = 0;
+    }
+    const int U = (int)total, before = (int)min(lead, (long long)kMaxUnits);
+    const int G = min((int)gridDim.x, U);
+    const int c = blockIdx.x;
+    const int u0 = c < G ? (int)((long long)c * U / G) : 0, u1 = c < G ? (int)((long long)(c + 1) * U / G) : 0;
+    if (u0 < u1 && u0 >= before && u0 < before + mine) {
+        int pre = before;
+        for (int b = rb0; b < rb1; b++) {
+            const Req r = request(a, b);
+            if (u0 < pre + r.items * r.tiles) { s_cur[0] = b; s_cur[1] = pre; break; }
+            pre += r.items * r.tiles;
         }
     }
-    float m = -INFINITY, l = 0.f;
-    for (int t0 = 0; t0 < seen; t0 += 16) {
-        __syncthreads();
-        // a tile never crosses a page (page % 16 == 0)
-        const int pg = a.table[(size_t)b * a.max_pages + t0 / a.d.page];
-        const bool ok = pg >= 0 && pg < a.d.n_pages;
-        if (!ok && threadIdx.x == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, pg, 3);
-        const int tn = ok ? min(16, seen - t0) : 0;
-        const uint8_t *base = a.d.p + (size_t)(ok ? pg : 0) * a.d.page_bytes;
-        const int in0 = t0 % a.d.page;
-        for (int i = threadIdx.x; i < tn * W; i += blockDim.x) {
-            const int r = i / W, c = i % W, in = in0 + r;
-            const uint32_t eb = base[a.d.o_exp + in];
-            const float unit = eb == 255u ? __uint_as_float(0x7fc00000u) : e8m0_to_f32(eb);
-            float v;
-            if (c < a.d.kv) {
-                const uint32_t byte = base[(size_t)in * (a.d.kv / 2) + c / 2];
-                const float2 f = f16x2_to_f32x2(e2m1x2_to_f16x2(byte));
-                v = (c & 1 ? f.y : f.x) * e4m3_to_f32(base[a.d.o_scale + in * (a.d.kv / 16) + c / 16]);
-            } else {
-                v = __half2float(reinterpret_cast<const __half *>(base + a.d.o_rope)[in * a.d.rope + c - a.d.kv]);
+    __syncthreads();
+    Cursor cur;
+    cur.u = u0;
+    cur.u1 = u1;
+    cur.b = 0; cur.pre = 0;
+    if (u0 < u1) {
+        cur.b = s_cur[0];
+        cur.pre = s_cur[1];
+        cur.r = request(a, cur.b);
+    }
+    if (tid == 0) {
+        int4 i0 = make_int4(u0, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
+        Cursor t = cur;
+        Seg s;
+        if (next_seg(a, t, s)) {
+            i0 = make_int4(u0, s.begin, s.end, 0);
+            i1 = make_int4(s.row0, s.rows, 0, 0);
+        } else {
+            i0.x = 0x7fffffff;
+        }
+        a.info[2 * c] = i0;
+        a.info[2 * c + 1] = i1;
+    }
+    const uint32_t sq = base + L.q, sk = base + L.k, sp = base + L.p;
+    const uint32_t t_o = tmem + 128;                      // S at columns 0 and 64, O^T behind
+    Seg s;
+    int item = 0, g = 0;                                  // items and tiles so far (barrier phases)
+
+    if (warp < 8) {
+        // ------------------------------------------------------------------- widening
+        const int row = tid >> 2, part = tid & 3;
+        while (next_seg(a, cur, s)) {
+            const bool any = s.t0 < s.t1;
+            Raw<NB> nx;
+            int pg = -1;
+            if (any) {
+                pg = page_at(a, s.b, s.t0 * kT + row, s.kvl);
+                load_raw<NB>(nx, a, pg, s.t0 * kT + row, part);
+                pg = s.t0 + 1 < s.t1 ? page_at(a, s.b, (s.t0 + 1) * kT + row, s.kvl) : -1;
             }
-            tile[r][c] = v * unit;
+            if (item > 0 && !mbar_wait(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) break;
+            load_q(a, s, sq, fac, lim, warp, lane);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_qfull);
+            item++;
+            bool stop = false;
+            for (int t = s.t0; t < s.t1; t++, g++) {
+                const Raw<NB> r = nx;
+                if (t + 1 < s.t1) {
+                    load_raw<NB>(nx, a, pg, (t + 1) * kT + row, part);
+                    pg = t + 2 < s.t1 ? page_at(a, s.b, (t + 2) * kT + row, s.kvl) : -1;
+                }
+                const int buf = g & 1;
+                if (g >= 2 && !mbar_wait(b_pv + 8 * buf, ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { stop = true; break; }
+                widen<NB>(r, sk + (uint32_t)buf * panels * kPanel, row, part, a.d.rope);
+                if (part == 0) {
+                    // e; NaN for a row of NaN, minus infinity where there is none
+                    kinfo[buf * kT + row] = r.e < 0 ? __int_as_float(0xff800000)
+                                          : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(r.e - 127);
+                }
+                async_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_kfull + 8 * buf);
+            }
+            if (stop) break;
         }
-        __syncthreads();
-        for (int r = 0; r < tn; r++) {
-            float s = 0.f;
+    } else if (warp == 12) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            const uint32_t id_s = idesc(64, kT, 0);
+            bool stop = false;
+            auto scores = [&](int k) -> bool {            // S of the k-th tile of this CTA
+                const int buf = k & 1;
+                if (!mbar_wait(b_kfull + 8 * buf, (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+                tc_after();
+                const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, d = tmem + (uint32_t)(buf * kT);
+                for (int p = 0; p < NB * 2; p++)
 #pragma unroll
-            for (int i = 0; i < 18; i++)
-                if (lane + 32 * i < W) s = fmaf(q[i], tile[r][lane + 32 * i], s);
-            s = warp_sum(s) * a.scale;
-            const float mn = fmaxf(m, s);
-            const float f = m == -INFINITY ? 0.f : expf(m - mn);
-            const float p = s == -INFINITY ? 0.f : expf(s - mn);
-            l = l * f + p;
+                    for (int k4 = 0; k4 < 4; k4++)
+                        mma(d, desc_k(sq + p * kPanel + 32u * k4), desc_k(tile + p * kPanel + 32u * k4), id_s, (p | k4) ? 1u : 0u);
+                for (int k4 = 0; k4 < a.d.rope / 16; k4++)
+                    mma(d, desc_k(sq + NB * 2 * kPanel + 32u * k4), desc_k(tile + NB * 2 * kPanel + 32u * k4), id_s, 1u);
+                commit(b_sfull + 8 * buf);
+                return true;
+            };
+            while (!stop && next_seg(a, cur, s)) {
+                if (!mbar_wait(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
+                tc_after();
+                item++;
+                const int nt = max(0, s.t1 - s.t0);
+                if (nt == 0) {
+                    commit(b_qempty);
+                    continue;
+                }
+                const int NR = (s.rows + 15) & ~15;       // columns of O^T
+                const uint32_t id_o = idesc(128, NR, 1);
+                if (!scores(g)) break;
+                if (nt == 1) commit(b_qempty);
+                for (int i = 0; i < nt; i++, g++) {
+                    if (i + 1 < nt) {
+                        if (!scores(g + 1)) { stop = true; break; }
+                        if (i + 2 == nt) commit(b_qempty);
+                    }
+                    if (!mbar_wait(b_pfull, g & 1, abort, K3_SITE_CACHE4, 5, g)) { stop = true; break; }
+                    tc_after();
+                    const uint32_t tile = sk + (uint32_t)(g & 1) * panels * kPanel;
+                    for (int blk = 0; blk < NB; blk++)
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (lane + 32 * i < a.d.kv) acc[i] = fmaf(p, tile[r][lane + 32 * i], acc[i] * f);
-            m = mn;
+                        for (int k4 = 0; k4 < kT / 16; k4++)
+                            mma(t_o + (uint32_t)(blk * NR), desc_mn(tile + 2 * blk * kPanel + 2048u * k4, kPanel),
+                                desc_k(sp + 32u * k4), id_o, (i | k4) ? 1u : 0u);
+                    commit(b_pv + 8 * (g & 1));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // --------------------------------------------------- softmax, rescale, results
+        const int w = warp - 8, gr = lane >> 2, t4 = lane & 3;
+        const int ra = 16 * w + gr, rb = ra + 8;          // this thread's rows
+        const float NEG = __int_as_float(0xff800000);
+        const uint32_t lanes = (uint32_t)(32 * w) << 16;
+        bool dead = false;
+        int seg_no = 0;
+        while (next_seg(a, cur, s)) {
+            const bool slot1 = seg_no > 0;                // a later piece of this CTA
+            seg_no++;
+            if (item > 0 && !mbar_wait(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 6, item)) dead = true;
+            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_qfull);
+            if (!dead && !mbar_wait(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
+            item++;
+            const int NR = (s.rows + 15) & ~15;
+            const float fa = fac[ra], fb = fac[rb];
+            const int la = lim[ra], lb = lim[rb];
+            float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
+            bool leave = false;
+            for (int t = s.t0; t < s.t1; t++, g++) {
+                const int buf = g & 1;
+                if (!dead && !(mbar_wait(b_kfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                               mbar_wait(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
+                    dead = true;
+                tc_after();
+                float v[32];
+                ld_s(tmem + lanes + (uint32_t)(buf * kT), v);
+                const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
+                // s (base 2) stays in v; the largest s + e of the tile
+                float xa = NEG, xb = NEG;
+                float ke[16];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 k = ki[4 * i + t4];      // e of two neighbouring positions
+                    const float u0 = unit(k.x), u1 = unit(k.y);
+                    const int pos = t * kT + 8 * i + 2 * t4;
+                    ke[2 * i] = k.x;
+                    ke[2 * i + 1] = k.y;
+                    const bool h0 = k.x != NEG, h1 = k.y != NEG;
+                    v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
+                    v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
+                    v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
+                    v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
+                    xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
+                    xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
+                }
+                xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
+                xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
+                xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
+                xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
+                // move the references; a row's accumulator changes only if it held something
+                float ca = 1.f, cb = 1.f;
+                if (ma == NEG) ma = xa;
+                else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
+                if (mb == NEG) mb = xb;
+                else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
+                const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
+                const bool move = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
+                if (lane == 0) flags[buf * 4 + w] = (move ? 1 : 0) | (dead ? 2 : 0);
+                uint32_t pa[8], pb[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float e0 = ke[2 * i], e1 = ke[2 * i + 1];
+                    suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
+                    sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
+                    // a masked position is minus infinity whatever its e is
+                    const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + e0 - na);
+                    const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + e1 - na);
+                    const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + e0 - nb);
+                    const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + e1 - nb);
+                    const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                    pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                    pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                }
+                // O(t - 1) has been added: P may be written, and the accumulator rescaled
+                if (t > s.t0 && !dead && !mbar_wait(b_pv + 8 * (buf ^ 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                tc_after();
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
+                }
+                if (t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
+                named_sync(1, 128);
+                const int4 fl = *reinterpret_cast<const int4 *>(flags + buf * 4);
+                const int f = fl.x | fl.y | fl.z | fl.w;
+                if (f & 2) { leave = true; break; }
+                if ((f & 1) && t > s.t0) {
+                    for (int blk = 0; blk < NB; blk++)
+                        for (int c0 = 0; c0 < NR; c0 += 16) {
+                            float o[16];
+                            ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] *= rowf[c0 + i];
+                            st16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+                        }
+                }
+                if (f & 1) named_sync(1, 128);            // rowf is rewritten by the next tile
+                async_fence();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_pfull);
+            }
+            if (leave) break;
+            // ---- the item's result
+            suma += __shfl_xor_sync(0xffffffffu, suma, 1);
+            sumb += __shfl_xor_sync(0xffffffffu, sumb, 1);
+            suma += __shfl_xor_sync(0xffffffffu, suma, 2);
+            sumb += __shfl_xor_sync(0xffffffffu, sumb, 2);
+            const bool any = s.t0 < s.t1;
+            const size_t slot = (size_t)c * 2 + (slot1 ? 1 : 0);
+            if (t4 == 0) {
+                if (s.whole) {
+                    rowf[ra] = suma == 0.f ? 0.f : 1.f / suma;
+                    rowf[rb] = sumb == 0.f ? 0.f : 1.f / sumb;
+                } else {
+                    a.ml[slot * kR + ra] = make_float2(ma, suma);
+                    a.ml[slot * kR + rb] = make_float2(mb, sumb);
+                }
+            }
+            if (any && !dead && !mbar_wait(b_pv + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            tc_after();
+            named_sync(1, 128);
+            const int kv = NB * 128;
+            for (int blk = 0; blk < NB && !dead; blk++) {
+                const int col = blk * 128 + 32 * w + lane;
+                for (int c0 = 0; c0 < s.rows; c0 += 16) {
+                    float o[16];
+                    if (any) {
+                        ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[i] = 0.f;
+                    }
+                    if (s.whole) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (c0 + i < s.rows) {
+                                const size_t at = (size_t)(s.row0 + c0 + i) * kv + col;
+                                const float r = o[i] * rowf[c0 + i];
+                                if (a.out_f32) ((float *)a.out)[at] = r;
+                                else ((uint16_t *)a.out)[at] = f32_to_bf16_bits(r);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (c0 + i < s.rows) a.part[(slot * kR + c0 + i) * kv + col] = o[i];
+                    }
+                }
+            }
+            tc_before();
+            named_sync(1, 128);                           // rowf is free again, O^T is read
         }
     }
-    if (h >= a.H) return;
-    const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int c = lane + 32 * i;
-        if (c < a.d.kv) {
-            const size_t at = ((size_t)n * a.H + h) * a.d.kv + c;
-            if (a.out_f32) ((float *)a.out)[at] = acc[i] * inv;
-            else ((uint16_t *)a.out)[at] = f32_to_bf16_bits(acc[i] * inv);
+    __syncthreads();
+    if (warp == 12 && lane == 0) {
+        // every MMA issued above has completed once this barrier flips
+        commit(b_drain);
+        const long long t0 = clock64();
+        while (!mbar_try(b_drain, 0)) {
+            if (clock64() - t0 > kSpinLimit) { k3_raise_at(K3D_ETIMEOUT, K3_SITE_CACHE4, 12, 0, (int)blockIdx.x); break; }
+        }
+    }
+    __syncthreads();
+    if (warp == 12) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+    }
+}
+
+// The pieces of each cut item, added in CTA order. Block (k, row): the k-th cut item (an item
+// is led by the first CTA boundary inside it), one of its rows; thread t has the columns
+// 4 t .. 4 t + 3 of every piece.
+__global__ void __launch_bounds__(128) k_attend4_merge(const Args a, int grid)
+{
+    __shared__ int s_c;
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) s_c = -1;
+    __syncthreads();
+    if (tid < 32) {
+        int found = 0;
+        for (int c0 = 1; c0 < grid; c0 += 32) {
+            const int c = c0 + lane;
+            bool lead = false;
+            if (c < grid) {
+                const int4 i = a.info[2 * c];
+                lead = i.y >= 0 && i.y < i.x && a.info[2 * (c - 1)].x <= i.y;
+            }
+            const unsigned m = __ballot_sync(0xffffffffu, lead);
+            const int rank = found + __popc(m & ((1u << lane) - 1u));
+            if (lead && rank == (int)blockIdx.x) s_c = c;
+            found += __popc(m);
+        }
+    }
+    __syncthreads();
+    const int c = s_c;
+    if (c < 0) return;
+    const int4 i0 = a.info[2 * c], i1 = a.info[2 * c + 1];
+    const int r = blockIdx.y;
+    if (r >= i1.y) return;
+    const int end = i0.z;
+    // pieces: CTA c - 1 (its second slot unless the item begins its range), then c, c + 1, ...
+    int last = c;
+    while (last + 1 < grid && a.info[2 * (last + 1)].x < end) last++;
+    const int np = last - c + 2;
+    const size_t first = (size_t)(c - 1) * 2 + (a.info[2 * (c - 1)].x == i0.y ? 0 : 1);
+    auto slot = [&](int k) { return k == 0 ? first : (size_t)(c - 1 + k) * 2; };
+    const int kv = a.d.kv;
+    float M = __int_as_float(0xff800000);
+    for (int k = 0; k < np; k++) {
+        const float m = a.ml[slot(k) * kR + r].x;
+        M = m > M || m != m ? m : M;
+    }
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const bool on = tid * 4 < kv;
+#pragma unroll 4
+    for (int k = 0; k < np; k++) {
+        const float2 ml = a.ml[slot(k) * kR + r];
+        if (ml.x == __int_as_float(0xff800000) && ml.y == 0.f) continue;
+        const float f = exp2f(ml.x - M);
+        l += ml.y * f;
+        if (on) {
+            const float4 o = *reinterpret_cast<const float4 *>(a.part + (slot(k) * kR + r) * kv + tid * 4);
+            acc.x = fmaf(o.x, f, acc.x);
+            acc.y = fmaf(o.y, f, acc.y);
+            acc.z = fmaf(o.z, f, acc.z);
+            acc.w = fmaf(o.w, f, acc.w);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (on) {
+        const size_t at = (size_t)(i1.x + r) * kv + tid * 4;
+        acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+        if (a.out_f32) {
+            *reinterpret_cast<float4 *>((float *)a.out + at) = acc;
+        } else {
+            uint2 u;
+            u.x = (uint32_t)f32_to_bf16_bits(acc.x) | ((uint32_t)f32_to_bf16_bits(acc.y) << 16);
+            u.y = (uint32_t)f32_to_bf16_bits(acc.z) | ((uint32_t)f32_to_bf16_bits(acc.w) << 16);
+            *reinterpret_cast<uint2 *>((uint16_t *)a.out + at) = u;
         }
     }
 }
 
-}  // namespace
+static int grid_size() { return sm_count() > 0 ? sm_count() : 148; }
+
+static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+struct Ws {
+    size_t part, ml, info, total;
+};
+
+static Ws ws_layout(int kv)
+{
+    const size_t g = grid_size();
+    Ws w;
+    w.part = 0;
+    w.ml = al256(g * 2 * kR * kv * sizeof(float));
+    w.info = w.ml + al256(g * 2 * kR * sizeof(float2));
+    w.total = w.info + al256(g * 2 * sizeof(int4));
+    return w;
+}
+
+template <int NB>
+static cudaError_t launch(const Args &a, int grid, size_t smem, cudaStream_t st)
+{
+    static unsigned long long init = 0;   // one bit per device
+    if (!(init & dev_bit())) {
+        allow_smem_max(k_attend4<NB>);
+        init |= dev_bit();
+    }
+    return launch_pdl(k_attend4<NB>, dim3(grid), dim3(kThreads), smem, st, a);
+}
+
+}  // namespace at4
 }  // namespace k3
 
 using namespace k3;
@@ -126,7 +913,7 @@ extern "C" {
 size_t k3d_mla_attend4_ws_bytes(const K3dCache4 *c, int B, int N, int H)
 {
     if (cache4_check(c, "k3d_mla_attend4_ws_bytes") || B < 1 || N < 0 || H < 1) return 0;
-    return 256;
+    return at4::ws_layout(c->kv_lora).total;
 }
 
 int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const K3dCache4 *c, const void *pool,
@@ -134,7 +921,8 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
                     float scale, void *ws, size_t ws_bytes)
 {
     K3_TRY(cache4_check(c, "k3d_mla_attend4"));
-    if (B < 1 || N < 0 || H < 1 || H > 1024 || max_pages < 1 || (long long)max_pages * c->page > 0x7fffffffLL)
+    if (B < 1 || N < 0 || H < 1 || H > 1024 || max_pages < 1 || (long long)max_pages * c->page > 0x7fffffffLL ||
+        (long long)N * H > 0x7fffffffLL)
         return fail(K3D_EINVAL, "k3d_mla_attend4: B %d, N %d, H %d (1 to 1024), max_pages %d", B, N, H, max_pages);
     for (int t : {out_dtype, q_dtype})
         if (t != K3D_DT_F32 && t != K3D_DT_BF16)
@@ -148,11 +936,30 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
         return fail(K3D_EINVAL, "k3d_mla_attend4: unaligned table, row_start or kv_len");
     if (ws_bytes < k3d_mla_attend4_ws_bytes(c, B, N, H)) return fail(K3D_EINVAL, "k3d_mla_attend4 workspace");
     K3_TRY(ensure_ctx());
-    const Attend a{pool4(c, pool), q, out, table, row_start, kv_len, max_pages, B, N, H,
-                   q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, scale};
-    launch_pdl(k_attend4_plain, dim3(N, (H + 7) / 8), dim3(256), 0, stream(), a);
+    const at4::Ws w = at4::ws_layout(c->kv_lora);
+    char *wb = (char *)ws;
+    const at4::Args a{pool4(c, pool), q, out, table, row_start, kv_len, max_pages, B, N, H,
+                      q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, scale,
+                      (float *)(wb + w.part), (float2 *)(wb + w.ml), (int4 *)(wb + w.info)};
+    const int grid = at4::grid_size();
+    const size_t smem = 1024 + at4::smem_layout(c->kv_lora, c->qk_rope).total;
+    switch (c->kv_lora / 128) {
+    case 1: at4::launch<1>(a, grid, smem, stream()); break;
+    case 2: at4::launch<2>(a, grid, smem, stream()); break;
+    case 3: at4::launch<3>(a, grid, smem, stream()); break;
+    default: at4::launch<4>(a, grid, smem, stream()); break;
+    }
     note_launch();
-    return check_launch("mla attend4");
+    K3_TRY(check_launch("mla attend4"));
+    // at most one cut item per CTA boundary, and no more than there are items
+    const long long items = H <= at4::kR ? N : (long long)N * ((H + at4::kR - 1) / at4::kR);
+    const int cuts = (int)(items < grid - 1 ? items : grid - 1);
+    if (cuts > 0) {
+        launch_pdl(at4::k_attend4_merge, dim3(cuts, H < at4::kR ? (at4::kR / H) * H : at4::kR), dim3(128), 0, stream(), a, grid);
+        note_launch();
+        K3_TRY(check_launch("mla attend4 merge"));
+    }
+    return K3D_OK;
 }
 
 }  // extern "C"

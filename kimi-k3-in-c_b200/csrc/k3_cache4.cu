@@ -34,12 +34,12 @@ __device__ __forceinline__ void load_n(float *v, const float *src)
     if (VEC) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const float4 t = __ldg(reinterpret_cast<const float4 *>(src) + i);
+            const float4 t = reinterpret_cast<const float4 *>(src)[i];
             v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = __ldg(src + i);
+        for (int i = 0; i < N; i++) v[i] = src[i];
     }
 }
 
@@ -49,7 +49,7 @@ __device__ __forceinline__ void load_n(float *v, const uint16_t *src)
     if (VEC) {
 #pragma unroll
         for (int i = 0; i < N / 8; i++) {
-            const uint4 t = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+            const uint4 t = reinterpret_cast<const uint4 *>(src)[i];
             const uint32_t u[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -59,7 +59,7 @@ __device__ __forceinline__ void load_n(float *v, const uint16_t *src)
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = bf16_to_f32(__ldg(src + i));
+        for (int i = 0; i < N; i++) v[i] = bf16_to_f32(src[i]);
     }
 }
 
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const 
     const int lane = threadIdx.x & 31;
     const int r = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     if (r >= N) return;
-    const int slot = __ldg(slots + r);
+    const int slot = slots[r];
     if (slot < 0 || slot >= d.n_pages * d.page) {
         if (slot != -1 && lane == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, r, slot, 0);
         return;
@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const 
     for (int i = 0; i < 16; i++) v[i] = 0.f;
     if (own) load_n<VEC, 16>(v, src + lane * 16);
     if (ropes) {
-        rv[0] = to_f(__ldg(src + d.kv + 2 * lane));
-        rv[1] = to_f(__ldg(src + d.kv + 2 * lane + 1));
+        rv[0] = to_f(src[d.kv + 2 * lane]);
+        rv[1] = to_f(src[d.kv + 2 * lane + 1]);
     }
     float amax = 0.f, rmax = fmaxf(fabsf(rv[0]), fabsf(rv[1]));
     bool fine = fabsf(rv[0]) <= 3.4028234e38f && fabsf(rv[1]) <= 3.4028234e38f;
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_load(Pool4 d, T *out,
     const int lane = threadIdx.x & 31;
     const int r = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     if (r >= N) return;
-    const int slot = __ldg(slots + r);
+    const int slot = slots[r];
     if (slot < 0 || slot >= d.n_pages * d.page) {
         if (slot != -1 && lane == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, r, slot, 1);
         return;

@@ -136,7 +136,7 @@ class Batch:
         ids = first_page + g.permutation(n_pages - first_page)
         self.max_pages = max(need + [1]) + 1
         self.table = np.full((len(reqs), self.max_pages), -1, np.int32)
-        self.values, at = [], 0
+        self.values, self.exps, at = [], [], 0
         for b, (k, _) in enumerate(reqs):
             self.table[b, :need[b]] = ids[at:at + need[b]]
             at += need[b]
@@ -147,7 +147,9 @@ class Batch:
             slots = (self.table[b, t // page] * page + t % page).astype(np.int32)
             if k:
                 store(lib, self.shape, self.pool, x, slots)
-            self.values.append(ref.quantise(x, kv)[1])
+            fields, value = ref.quantise(x, kv)
+            self.values.append(value)
+            self.exps.append(fields[3].astype(int) - 127)
         self.start = np.concatenate([[0], np.cumsum([n for _, n in reqs])]).astype(np.int32)
         self.bufs = [i32(self.table), i32(self.start), i32([k for k, _ in reqs])]
         self.g = g
@@ -175,7 +177,11 @@ class Batch:
     def compare(self, got, q, H, qt, ot, scale):
         """Elementwise: half a step of the result's type, the weights' rounding to fp16 (2^-11 of
         sum p|v|), q's rounding to fp16 where it is fp32 and the fp32 sums of 576 products
-        (both as a change of the scores), and 2^-16 of sum p|v| for exp2 and the running sums."""
+        (both as a change of the scores), and 2^-16 of sum p|v| for exp2 and the running sums.
+        Small weights: the kernel rounds P = 2^(a - m + 7), a = s + e (base 2), m <= max a, to
+        fp16, whose steps stop at 2^-24, so P is off by up to 2^-25 however small it is. With
+        L = sum 2^(s - m + 7) >= 2^(7 - e*), e* the unit of the position of max a, the result
+        sum P (v 2^-e) / L moves by at most 2^-32 sum |v| 2^(e* - e)."""
         eps = 2.0 ** -8 if ot == BF16 else 2.0 ** -24
         for b, (k, n) in enumerate(self.reqs):
             v = self.values[b]
@@ -192,7 +198,9 @@ class Batch:
                 p /= p.sum(1, keepdims=True)
                 mag = p @ np.abs(v[:seen, :self.kv])
                 ds = scale * (np.abs(x) @ np.abs(v[:seen]).T).max(1) * ((2.0 ** -11 if qt == F32 else 0.0) + 576 * 2.0 ** -24)
-                tol = eps * np.abs(want[j]) + (2.0 ** -11 + 2.0 ** -16 + np.expm1(2 * ds))[:, None] * mag
+                top = self.exps[b][(s * np.log2(np.e) + self.exps[b][:seen]).argmax(1)]
+                low = 2.0 ** -32 * np.exp2(top[:, None]) * (np.abs(v[:seen, :self.kv]) * np.exp2(-1.0 * self.exps[b][:seen, None])).sum(0)
+                tol = eps * np.abs(want[j]) + (2.0 ** -11 + 2.0 ** -16 + np.expm1(2 * ds))[:, None] * mag + low
                 err = np.abs(got[s0 + j] - want[j])
                 assert (err <= tol).all(), (b, j, float((err / tol).max()))
 
@@ -298,6 +306,7 @@ def test_attend_pages_outside_the_pool(k3):
     assert k3.k3d_sync() == k3cuda.K3D_EDEVICE
     k3.k3d_clear_status()
     B.values[0] = np.concatenate([B.values[0][:64], B.values[0][128:]])
+    B.exps[0] = np.concatenate([B.exps[0][:64], B.exps[0][128:]])
     B.reqs = [(136, 1)]
     B.compare(got, q, 64, BF16, F32, 0.07)
 
