@@ -15,23 +15,31 @@
 // (unnormalised o, max, sum) and a second kernel adds them in CTA order.
 //
 // PRODUCTS (tcgen05, fp16 x fp16, fp32 accumulators in tensor memory). A tile's rows are
-// widened once to fp16 in units of 2^e (exact, k3_cache4.cuh), 64 values to a 128-byte
-// swizzled panel row, and serve both products from the same bytes:
+// widened once to fp16, 64 values to a 128-byte swizzled panel row, and serve both products
+// from the same bytes:
 //   S [64 rows][64 keys]     = Q K^T      M = 64, K-major A = Q and B = the tile
 //   O^T [kv][rows] (4 x 128) += V^T P^T   M = 128 latents, A = the tile read MN-major,
 //                                         B = P, K-major, N = the rows rounded up to 16
 // O^T rather than O keeps the accumulator of 64 rows in 256 of the 512 columns, which leaves
-// room for two S; O of 64 rows and 512 latents would fill all of them. q is fp16 in units of
-// its row (exact for bf16 within 2^-29 of the row's largest value). The softmax works on
-// a = s log2(e) + e: P = 2^(a - m), rounded to fp16 (2^-12 on average, an eighth of the step
-// of a bf16 result), carries the key's unit 2^e, while the sum takes 2^(s - m) in fp32. m is
-// a reference that moves only when a tile's maximum passes it by 2^8, so that the
-// accumulator is rescaled rarely; P is kept below 2^15 and weights down to 2^-31 of the
-// largest keep their value.
+// room for two S; O of 64 rows and 512 latents would fill all of them.
+//
+// UNITS. The fp16 operand holds values in units of 2^-2. A stored row is a multiple of 2^-10
+// of its own 2^e, so for -16 <= e <= -2 (largest latent between 0.02 and 672) the step to
+// 2^-2 is exact in fp16. A row outside keeps a residual 2^r in fp32: its scores are
+// multiplied by it, and its weight P carries it into the second product, so that rows of any
+// size stay exact. q is fp16 in units of its row (exact for bf16 within 2^-29 of the row's
+// largest value).
+//
+// SOFTMAX. With a = s log2(e) + r: P = 2^(a - m + 7), rounded to fp16 (half a step is 2^-12
+// on average, an eighth of a bf16 result's), and the sum takes 2^(a - r - m + 7) in fp32. m
+// moves only when a tile's maximum passes it by 2^8, so the accumulator is rescaled rarely;
+// P stays below 2^15 and weights down to 2^-21 of the largest keep all their bits.
 //
 // ROLES (416 threads): warps 0-7 load a tile ahead into registers, widen and store it;
-// warps 8-11 do the softmax, the rescaling and the results; warp 12 issues the MMAs, in the
-// order S(t + 1), O(t). All 12 load Q. Every wait is bounded (k3_bulk.cuh).
+// warps 8-11 do the softmax and the rescaling; these 12 load Q and write the results; warp
+// 12 issues the MMAs, tiles in pairs: S(t), S(t + 1), O(t), O(t + 1), so that the softmax of
+// one tile and the widening of the next pair run under the other's products. Every wait is
+// bounded (k3_bulk.cuh).
 #include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"
@@ -48,6 +56,9 @@ constexpr int kThreads = 416;
 constexpr int kMaxUnits = 1 << 30;
 constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
 constexpr float kStep = 8.f;              // m moves when a tile passes it by this
+constexpr int kUnit = -2;                 // the fp16 operand is in units of 2^kUnit
+constexpr int kDown = 14;                 // a row's 2^e is taken into fp16 for kUnit - 14 <= e <= kUnit
+constexpr float kUnitF = 0.25f;
 
 struct Args {
     Pool4 d;
@@ -57,7 +68,7 @@ struct Args {
     int max_pages, B, N, H;
     int q_f32, out_f32;
     float scale;
-    float *part;                          // [grid][2][64][kv]
+    float *part;                          // [grid][2][kv / 32][16][32][4]: latent block, row / 4, latent, row % 4
     float2 *ml;                           // [grid][2][64] (max, sum), base 2
     int4 *info;                           // [grid][2]: {u0, item begin, item end, 0}, {row0, rows, 0, 0}
 };
@@ -73,16 +84,16 @@ __host__ __device__ inline Smem smem_layout(int kv, int rope)
     s.q = 0;
     s.k = s.q + panels * kPanel;
     s.p = s.k + 2 * panels * kPanel;
-    s.kinfo = s.p + kR * 128;             // float [2][64]: e of each position
+    s.kinfo = s.p + kR * 128;             // float [2][64]: residual of each position
     s.row = s.kinfo + 2 * kT * 4;         // float [64] score factor, int [64] limit, float [64] x 2
     s.bars = s.row + 4 * kR * 4;
-    s.total = s.bars + 160;
+    s.total = s.bars + 160 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
     return s;
 }
 
 // One request as the scheduler sees it.
 struct Req {
-    int n, kvl, items, tiles;
+    int first, n, kvl, items, tiles;
 };
 
 __device__ __forceinline__ Req request(const Args &a, int b)
@@ -96,6 +107,7 @@ __device__ __forceinline__ Req request(const Args &a, int b)
         if (r0 < 0 || n < 0 || r1 > a.N) n = 0;
         kvl = max(0, min(kvl, cap));
     }
+    r.first = r0;
     r.n = n;
     r.kvl = kvl;
     const int per = a.H <= kR ? kR / a.H : 1;
@@ -133,7 +145,7 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
     s.kvl = c.r.kvl;
     s.begin = c.pre + item * c.r.tiles;
     s.end = s.begin + c.r.tiles;
-    const int first = a.row_start[c.b];
+    const int first = c.r.first;
     int last;
     if (a.H <= kR) {
         const int per = kR / a.H;
@@ -185,17 +197,36 @@ __device__ __forceinline__ uint32_t idesc(int M, int N, int a_mn)
     return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
+// The whole warp runs the issue loop, so that addresses stay in uniform registers; `lead` is
+// one lane's.
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum, uint32_t lead)
 {
-    asm volatile("{\n\t.reg .pred p;\n\t"
+    asm volatile("{\n\t.reg .pred p, l;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum) : "memory");
+                 "setp.ne.b32 l, %5, 0;\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum), "r"(lead) : "memory");
 }
 
-__device__ __forceinline__ void commit(uint32_t bar)
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred l;\n\t"
+                 "setp.ne.b32 l, %1, 0;\n\t"
+                 "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 :: "r"(bar), "r"(lead) : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+
+// A whole warp's bounded wait: the lanes leave together, with the same answer.
+__device__ __forceinline__ bool wait_all(uint32_t b, uint32_t parity, volatile int *abort, int site, int who, int where)
+{
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, abort, site, who, where));
 }
 
 #define K3_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
@@ -257,7 +288,7 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint4 v)
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// 2^e of a whole e in [-126, 127] kept as a float: e + 127 lands in the low mantissa bits
+// 2^x of a whole x in [-126, 127] kept as a float: x + 127 lands in the low mantissa bits
 __device__ __forceinline__ float unit(float e)
 {
     return __uint_as_float(__float_as_uint(e + 12583039.0f) << 23);
@@ -329,10 +360,13 @@ template <int NB>
 __device__ __forceinline__ void widen(const Raw<NB> &r, uint32_t tile, int row, int part, int rope)
 {
     const bool swap = part & 2;
+    // 2^(e - kUnit), from 2^-14 to 1, as f16x2
+    const uint32_t up = (uint32_t)(min(max(r.e - 127 - kUnit, -kDown), 0) + 15) * 0x04000400u;
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         uint32_t s2;                      // the two scales as f16x2
         asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(s2) : "r"(r.scale[i]));
+        s2 = hmul2(s2, up);
         const uint32_t lo = __byte_perm(s2, s2, 0x1010), hi = __byte_perm(s2, s2, 0x3232);
         const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
         const uint32_t panel = tile + (uint32_t)(2 * i + (part >> 1)) * kPanel;
@@ -347,77 +381,147 @@ __device__ __forceinline__ void widen(const Raw<NB> &r, uint32_t tile, int row, 
         }
     }
     const uint32_t panel = tile + (uint32_t)(2 * NB) * kPanel;
-    if (part < rope / 8) sts16(panel + swz(row, part), r.rope[0]);
-    if (part + 4 < rope / 8) sts16(panel + swz(row, part + 4), r.rope[1]);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (part + 4 * i < rope / 8)
+            sts16(panel + swz(row, part + 4 * i), make_uint4(hmul2(r.rope[i].x, up), hmul2(r.rope[i].y, up),
+                                                             hmul2(r.rope[i].z, up), hmul2(r.rope[i].w, up)));
 }
 
 // ------------------------------------------------------------------------------- Q ----
-// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the row's largest value in
-// [2^13, 2^14)), the score factor and the number of positions the row sees.
-__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
+// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the
+// row's largest value in [2^13, 2^14)), the score factor and the number of positions the row
+// sees. Rows behind the last are zeros that see everything: they cost no case of their own.
+template <bool F32>
+__device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
 {
+    constexpr int RB = F32 ? 1 : 3;                       // rows in flight (36 registers or 24)
     const int W = a.d.kv + a.d.rope, chunks = W / 8;
-    for (int r = warp; r < kR; r += 12) {
-        if (r >= s.rows) {
-            if (lane == 0) { fac[r] = 0.f; lim[r] = 0; }
-            continue;
+    for (int r0 = warp; r0 < kR; r0 += 12 * RB) {
+        uint4 raw[RB][3][F32 ? 2 : 1];
+#pragma unroll
+        for (int i = 0; i < RB; i++) {
+            const int r = r0 + 12 * i;
+            const size_t at = (size_t)(s.row0 + r) * W;
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                const int ch = lane + 32 * c;
+                const uint4 *p = reinterpret_cast<const uint4 *>((const char *)a.q + (at + ch * 8) * (F32 ? 4 : 2));
+#pragma unroll
+                for (int k = 0; k < (F32 ? 2 : 1); k++)
+                    raw[i][c][k] = ch < chunks && r < s.rows ? p[k] : make_uint4(0u, 0u, 0u, 0u);
+            }
         }
-        const size_t at = (size_t)(s.row0 + r) * W;
-        float v[3][8];
 #pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const int ch = lane + 32 * c;
+        for (int i = 0; i < RB; i++) {
+            const int r = r0 + 12 * i;
+            if (r >= kR) break;
+            auto value = [&](int c, float v[8]) {
+                const uint4 x = raw[i][c][0], y = raw[i][c][F32 ? 1 : 0];
+                const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                if (F32) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[c][k] = 0.f;
-            if (ch < chunks) {
-                if (a.q_f32) {
-                    const float4 *p = reinterpret_cast<const float4 *>((const float *)a.q + at + ch * 8);
-                    const float4 x = p[0], y = p[1];
-                    v[c][0] = x.x; v[c][1] = x.y; v[c][2] = x.z; v[c][3] = x.w;
-                    v[c][4] = y.x; v[c][5] = y.y; v[c][6] = y.z; v[c][7] = y.w;
+                    for (int k = 0; k < 8; k++) v[k] = __uint_as_float(u[k]);
                 } else {
-                    const uint4 x = *reinterpret_cast<const uint4 *>((const uint16_t *)a.q + at + ch * 8);
-                    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        v[c][2 * k] = __uint_as_float(u[k] << 16);
-                        v[c][2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                        v[2 * k] = __uint_as_float(u[k] << 16);
+                        v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                    }
+                }
+            };
+            float m = 0.f;
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                float v[8];
+                value(c, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[k]));
+            }
+            m = warp_max(m);
+            int e = 0;
+            if (m > 0.f && m <= 3.4028234e38f) {
+                frexpf(m, &e);
+                e = max(e, -110);
+            }
+            // the sign of the scale goes into q, so that a larger product is a larger score
+            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                const int ch = lane + 32 * c;
+                if (ch < chunks) {
+                    float v[8];
+                    value(c, v);
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const __half2 t = __floats2half2_rn(v[2 * k] * up, v[2 * k + 1] * up);
+                        h[k] = *reinterpret_cast<const uint32_t *>(&t);
+                    }
+                    sts16(sq + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
+                }
+            }
+            if (lane == 0) {
+                // |scale| log2(e) 2^(e - 14 + kUnit), the power in two factors (it may be below -126)
+                const int k = e - 14 + kUnit, k1 = k >> 1;
+                fac[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
+                         __uint_as_float((uint32_t)(k - k1 + 127) << 23);
+                const int j = s.j0 + (a.H <= kR ? r / a.H : 0);
+                lim[r] = r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
+{
+    if (a.q_f32) load_q_rows<true>(a, s, sq, fac, lim, warp, lane);
+    else load_q_rows<false>(a, s, sq, fac, lim, warp, lane);
+}
+
+// This warp's third of an item's result: the 16-row groups sub, sub + 3, ... of its quarter of
+// the lanes (latents). A whole item: neighbouring lanes trade halves, so that each writes a
+// pair of latents of eight rows. A piece: as it lies, four rows to a 16-byte store.
+template <int NB>
+__device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t slot, uint32_t t_o, int NR, bool any,
+                                          const float *rowf, int warp, int lane)
+{
+    const int q = warp & 3, sub = warp >> 2, ng = NR / 16;
+    const uint32_t lanes = (uint32_t)(32 * q) << 16;
+    constexpr int kv = NB * 128;
+    for (int i = sub; i < NB * ng; i += 3) {
+        const int blk = i / ng, c0 = (i - blk * ng) * 16;
+        float o[16];
+        if (any) {
+            ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k++) o[k] = 0.f;
+        }
+        if (s.whole) {
+            const int col = blk * 128 + 32 * q + (lane & ~1), up = (lane & 1) * 8;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float give = (lane & 1) ? o[k] : o[k + 8];
+                const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+                const int r = c0 + k + up;
+                if (r < s.rows) {
+                    const float f = rowf[r];
+                    const float x = ((lane & 1) ? got : o[k]) * f, y = ((lane & 1) ? o[k + 8] : got) * f;
+                    const size_t at = (size_t)(s.row0 + r) * kv + col;
+                    if (a.out_f32) {
+                        *reinterpret_cast<float2 *>((float *)a.out + at) = make_float2(x, y);
+                    } else {
+                        *reinterpret_cast<uint32_t *>((uint16_t *)a.out + at) =
+                            (uint32_t)f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16);
                     }
                 }
             }
-        }
-        float m = 0.f;
+        } else {
+            float4 *dst = reinterpret_cast<float4 *>(a.part) + ((slot * (NB * 4) + blk * 4 + q) * 16 + c0 / 4) * 32 + lane;
 #pragma unroll
-        for (int c = 0; c < 3; c++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[c][k]));
-        m = warp_max(m);
-        int e = 0;
-        if (m > 0.f && m <= 3.4028234e38f) {
-            frexpf(m, &e);
-            e = max(e, -110);
-        }
-        const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-#pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const int ch = lane + 32 * c;
-            if (ch < chunks) {
-                uint32_t h[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const __half2 t = __floats2half2_rn(v[c][2 * k] * up, v[c][2 * k + 1] * up);
-                    h[k] = *reinterpret_cast<const uint32_t *>(&t);
-                }
-                sts16(sq + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
-            }
-        }
-        if (lane == 0) {
-            // scale log2(e) 2^(e - 14), the power in two factors (e - 14 may be below -126)
-            const int k = e - 14, k1 = k >> 1;
-            fac[r] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
-                     __uint_as_float((uint32_t)(k - k1 + 127) << 23);
-            const int j = s.j0 + (a.H <= kR ? r / a.H : 0);
-            lim[r] = max(0, s.kvl - s.n + j + 1);
+            for (int k = 0; k < 4; k++)
+                if (c0 + 4 * k < s.rows) dst[k * 32] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
     }
 }
@@ -427,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
 {
     extern __shared__ unsigned char smem_raw[];
     __shared__ long long red[13];
-    __shared__ int s_cur[2];
+    __shared__ int s_cur[8];
     const uint32_t raw = saddr(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char *gb = smem_raw + (base - raw);
@@ -443,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     const uint32_t b_drain = b_qfull + 72;
     volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 96);
     uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 100);
+    int *kplain = reinterpret_cast<int *>(gb + L.bars + 160);           // [2][8]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -501,7 +606,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         int pre = before;
         for (int b = rb0; b < rb1; b++) {
             const Req r = request(a, b);
-            if (u0 < pre + r.items * r.tiles) { s_cur[0] = b; s_cur[1] = pre; break; }
+            if (u0 < pre + r.items * r.tiles) { 
+                s_cur[0] = b; s_cur[1] = pre; s_cur[2] = r.first; s_cur[3] = r.n;
+                s_cur[4] = r.kvl; s_cur[5] = r.items; s_cur[6] = r.tiles;
+                break;
+            }
             pre += r.items * r.tiles;
         }
     }
@@ -513,9 +622,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     if (u0 < u1) {
         cur.b = s_cur[0];
         cur.pre = s_cur[1];
-        cur.r = request(a, cur.b);
+        cur.r.first = s_cur[2]; cur.r.n = s_cur[3]; cur.r.kvl = s_cur[4];
+        cur.r.items = s_cur[5]; cur.r.tiles = s_cur[6];
     }
-    if (tid == 0) {
+    if (tid == 12 * 32) {
         int4 i0 = make_int4(u0, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
         Cursor t = cur;
         Seg s;
@@ -536,7 +646,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     if (warp < 8) {
         // ------------------------------------------------------------------- widening
         const int row = tid >> 2, part = tid & 3;
+        bool dead = false;
         while (next_seg(a, cur, s)) {
+            const bool slot1 = item > 0;                  // a later piece of this CTA
             const bool any = s.t0 < s.t1;
             Raw<NB> nx;
             int pg = -1;
@@ -545,79 +657,89 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 load_raw<NB>(nx, a, pg, s.t0 * kT + row, part);
                 pg = s.t0 + 1 < s.t1 ? page_at(a, s.b, (s.t0 + 1) * kT + row, s.kvl) : -1;
             }
-            if (item > 0 && !mbar_wait(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) break;
-            load_q(a, s, sq, fac, lim, warp, lane);
+            if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) dead = true;
+            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
             async_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_qfull);
             item++;
-            bool stop = false;
-            for (int t = s.t0; t < s.t1; t++, g++) {
+            for (int t = s.t0; t < s.t1 && !dead; t++, g++) {
                 const Raw<NB> r = nx;
                 if (t + 1 < s.t1) {
                     load_raw<NB>(nx, a, pg, (t + 1) * kT + row, part);
                     pg = t + 2 < s.t1 ? page_at(a, s.b, (t + 2) * kT + row, s.kvl) : -1;
                 }
                 const int buf = g & 1;
-                if (g >= 2 && !mbar_wait(b_pv + 8 * buf, ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { stop = true; break; }
+                if (g >= 2 && !wait_all(b_pv + 8 * buf, ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
                 widen<NB>(r, sk + (uint32_t)buf * panels * kPanel, row, part, a.d.rope);
-                if (part == 0) {
-                    // e; NaN for a row of NaN, minus infinity where there is none
-                    kinfo[buf * kT + row] = r.e < 0 ? __int_as_float(0xff800000)
-                                          : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(r.e - 127);
-                }
+                // the residual; NaN for a row of NaN, minus infinity where there is none
+                const int e = r.e - 127;
+                const float res = r.e < 0 ? __int_as_float(0xff800000)
+                                : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(e - min(max(e, kUnit - kDown), kUnit));
+                if (part == 0) kinfo[buf * kT + row] = res;
+                const int plain = __all_sync(0xffffffffu, res == 0.f);
+                if (lane == 0) kplain[buf * 8 + warp] = plain;
                 async_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b_kfull + 8 * buf);
             }
-            if (stop) break;
+            named_sync(2, 384);                           // the item's sums are written, O^T is complete
+            tc_after();
+            if (!dead)
+                write_out<NB>(a, s, (size_t)c * 2 + (slot1 ? 1 : 0), t_o, (s.rows + 15) & ~15, any, rowf, warp, lane);
+            tc_before();
         }
     } else if (warp == 12) {
         // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            const uint32_t id_s = idesc(64, kT, 0);
-            bool stop = false;
-            auto scores = [&](int k) -> bool {            // S of the k-th tile of this CTA
-                const int buf = k & 1;
-                if (!mbar_wait(b_kfull + 8 * buf, (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
-                tc_after();
-                const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, d = tmem + (uint32_t)(buf * kT);
-                for (int p = 0; p < NB * 2; p++)
+        const uint32_t lead = elect();
+        const uint32_t id_s = idesc(64, kT, 0);
+        const uint32_t pan = (uint32_t)(NB * 2 + (a.d.rope ? 1 : 0)) * kPanel;
+        const int kr = a.d.rope / 16;
+        const uint32_t t_m = __shfl_sync(0xffffffffu, tmem, 0);
+        bool stop = false;
+        auto scores = [&](int k) -> bool {                // S of the k-th tile of this CTA
+            const int buf = k & 1;
+            if (!wait_all(b_kfull + 8 * buf, (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+            tc_after();
+            const uint32_t d = t_m + (uint32_t)(buf * kT);
+            const uint64_t da = desc_k(sq), db = desc_k(sk + (uint32_t)buf * pan);
 #pragma unroll
-                    for (int k4 = 0; k4 < 4; k4++)
-                        mma(d, desc_k(sq + p * kPanel + 32u * k4), desc_k(tile + p * kPanel + 32u * k4), id_s, (p | k4) ? 1u : 0u);
-                for (int k4 = 0; k4 < a.d.rope / 16; k4++)
-                    mma(d, desc_k(sq + NB * 2 * kPanel + 32u * k4), desc_k(tile + NB * 2 * kPanel + 32u * k4), id_s, 1u);
-                commit(b_sfull + 8 * buf);
-                return true;
-            };
-            while (!stop && next_seg(a, cur, s)) {
-                if (!mbar_wait(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
-                tc_after();
-                item++;
-                const int nt = max(0, s.t1 - s.t0);
-                if (nt == 0) {
-                    commit(b_qempty);
-                    continue;
+            for (int p = 0; p < NB * 2; p++)
+#pragma unroll
+                for (int k4 = 0; k4 < 4; k4++)
+                    mma(d, da + (p * kPanel + 32 * k4) / 16, db + (p * kPanel + 32 * k4) / 16, id_s, (p | k4) ? 1u : 0u, lead);
+#pragma unroll
+            for (int k4 = 0; k4 < 4; k4++)
+                if (k4 < kr) mma(d, da + (NB * 2 * kPanel + 32 * k4) / 16, db + (NB * 2 * kPanel + 32 * k4) / 16, id_s, 1u, lead);
+            commit(b_sfull + 8 * buf, lead);
+            return true;
+        };
+        while (!stop && next_seg(a, cur, s)) {
+            if (!wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
+            tc_after();
+            item++;
+            const int nt = __shfl_sync(0xffffffffu, max(0, s.t1 - s.t0), 0);
+            const int NR = __shfl_sync(0xffffffffu, (s.rows + 15) & ~15, 0);      // columns of O^T
+            if (nt == 0) commit(b_qempty, lead);
+            const uint32_t id_o = idesc(128, NR, 1);
+            for (int i0 = 0; i0 < nt && !stop; i0 += 2) {
+                const int two = min(2, nt - i0);
+                for (int k = 0; k < two; k++) {
+                    if (!scores(g + k)) { stop = true; break; }
+                    if (i0 + k + 1 == nt) commit(b_qempty, lead);
                 }
-                const int NR = (s.rows + 15) & ~15;       // columns of O^T
-                const uint32_t id_o = idesc(128, NR, 1);
-                if (!scores(g)) break;
-                if (nt == 1) commit(b_qempty);
-                for (int i = 0; i < nt; i++, g++) {
-                    if (i + 1 < nt) {
-                        if (!scores(g + 1)) { stop = true; break; }
-                        if (i + 2 == nt) commit(b_qempty);
-                    }
-                    if (!mbar_wait(b_pfull, g & 1, abort, K3_SITE_CACHE4, 5, g)) { stop = true; break; }
+                for (int k = 0; k < two && !stop; k++, g++) {
+                    if (!wait_all(b_pfull, g & 1, abort, K3_SITE_CACHE4, 5, g)) { stop = true; break; }
                     tc_after();
-                    const uint32_t tile = sk + (uint32_t)(g & 1) * panels * kPanel;
+                    const uint64_t da = desc_mn(sk + (uint32_t)(g & 1) * pan, kPanel), db = desc_k(sp);
+                    const uint32_t acc = i0 + k ? 1u : 0u;
+#pragma unroll
                     for (int blk = 0; blk < NB; blk++)
 #pragma unroll
                         for (int k4 = 0; k4 < kT / 16; k4++)
-                            mma(t_o + (uint32_t)(blk * NR), desc_mn(tile + 2 * blk * kPanel + 2048u * k4, kPanel),
-                                desc_k(sp + 32u * k4), id_o, (i | k4) ? 1u : 0u);
-                    commit(b_pv + 8 * (g & 1));
+                            mma(t_m + 128 + (uint32_t)(blk * NR), da + (2 * blk * kPanel + 2048 * k4) / 16, db + 2 * k4, id_o,
+                                k4 ? 1u : acc, lead);
+                    commit(b_pv + 8 * (g & 1), lead);
                 }
             }
         }
@@ -629,90 +751,120 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         const float NEG = __int_as_float(0xff800000);
         const uint32_t lanes = (uint32_t)(32 * w) << 16;
         bool dead = false;
-        int seg_no = 0;
         while (next_seg(a, cur, s)) {
-            const bool slot1 = seg_no > 0;                // a later piece of this CTA
-            seg_no++;
-            if (item > 0 && !mbar_wait(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 6, item)) dead = true;
+            const bool slot1 = item > 0;
+            if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 6, item)) dead = true;
             if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
             async_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_qfull);
-            if (!dead && !mbar_wait(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
+            if (!dead && !wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
             item++;
             const int NR = (s.rows + 15) & ~15;
             const float fa = fac[ra], fb = fac[rb];
             const int la = lim[ra], lb = lim[rb];
+            const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
-            bool leave = false;
             for (int t = s.t0; t < s.t1; t++, g++) {
                 const int buf = g & 1;
-                if (!dead && !(mbar_wait(b_kfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
-                               mbar_wait(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
+                if (!dead && !(wait_all(b_kfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                               wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
                     dead = true;
                 tc_after();
                 float v[32];
                 ld_s(tmem + lanes + (uint32_t)(buf * kT), v);
-                const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
-                // s (base 2) stays in v; the largest s + e of the tile
-                float xa = NEG, xb = NEG;
-                float ke[16];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float2 k = ki[4 * i + t4];      // e of two neighbouring positions
-                    const float u0 = unit(k.x), u1 = unit(k.y);
-                    const int pos = t * kT + 8 * i + 2 * t4;
-                    ke[2 * i] = k.x;
-                    ke[2 * i + 1] = k.y;
-                    const bool h0 = k.x != NEG, h1 = k.y != NEG;
-                    v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
-                    v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
-                    v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
-                    v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
-                    xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
-                    xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
-                }
-                xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
-                xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
-                xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
-                xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
-                // move the references; a row's accumulator changes only if it held something
+                const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
+                const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
+                const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
                 float ca = 1.f, cb = 1.f;
-                if (ma == NEG) ma = xa;
-                else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
-                if (mb == NEG) mb = xb;
-                else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
-                const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
-                const bool move = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
-                if (lane == 0) flags[buf * 4 + w] = (move ? 1 : 0) | (dead ? 2 : 0);
+                // moves the references to a tile's maxima; a row's accumulator changes only if
+                // it held something
+                auto move = [&](float xa, float xb) {
+                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
+                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
+                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
+                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
+                    if (ma == NEG) ma = xa;
+                    else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
+                    if (mb == NEG) mb = xb;
+                    else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
+                };
                 uint32_t pa[8], pb[8];
+                if (plain) {
+                    // every row sees the whole tile, no residuals: the product's maximum is the
+                    // score's, and the sum adds what P is rounded from
+                    float xa = fmaxf(v[0], v[1]), xb = fmaxf(v[2], v[3]);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float e0 = ke[2 * i], e1 = ke[2 * i + 1];
-                    suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
-                    sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
-                    // a masked position is minus infinity whatever its e is
-                    const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + e0 - na);
-                    const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + e1 - na);
-                    const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + e0 - nb);
-                    const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + e1 - nb);
-                    const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                    pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
-                    pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                    for (int i = 1; i < 8; i++) {
+                        xa = fmaxf(xa, fmaxf(v[4 * i], v[4 * i + 1]));
+                        xb = fmaxf(xb, fmaxf(v[4 * i + 2], v[4 * i + 3]));
+                    }
+                    move(xa * fa, xb * fb);
+                    const float na = kLift - (ma == NEG ? 0.f : ma), nb = kLift - (mb == NEG ? 0.f : mb);
+                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float p0 = ex2(fmaf(v[4 * i], fa, na)), p1 = ex2(fmaf(v[4 * i + 1], fa, na));
+                        const float p2 = ex2(fmaf(v[4 * i + 2], fb, nb)), p3 = ex2(fmaf(v[4 * i + 3], fb, nb));
+                        s0 += p0; s1 += p1; s2 += p2; s3 += p3;
+                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                    }
+                    suma += s0 + s1;
+                    sumb += s2 + s3;
+                } else {
+                    const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
+                    float xa = NEG, xb = NEG;
+                    float kr[16];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float2 k = ki[4 * i + t4];  // residuals of two neighbouring positions
+                        const float u0 = unit(k.x), u1 = unit(k.y);
+                        const int pos = t * kT + 8 * i + 2 * t4;
+                        kr[2 * i] = k.x;
+                        kr[2 * i + 1] = k.y;
+                        const bool h0 = k.x != NEG, h1 = k.y != NEG;
+                        v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
+                        v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
+                        v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
+                        v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
+                        xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
+                        xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
+                    }
+                    move(xa, xb);
+                    const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float r0 = kr[2 * i], r1 = kr[2 * i + 1];
+                        suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
+                        sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
+                        // a masked position is minus infinity whatever its residual is
+                        const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + r0 - na);
+                        const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + r1 - na);
+                        const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + r0 - nb);
+                        const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + r1 - nb);
+                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                    }
                 }
+                const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
+                if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
                 // O(t - 1) has been added: P may be written, and the accumulator rescaled
-                if (t > s.t0 && !dead && !mbar_wait(b_pv + 8 * (buf ^ 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * (buf ^ 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
                 tc_after();
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
                     asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
                 }
-                if (t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
+                if (moved && t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
+                if (!moved && t4 == 0) { rowf[ra] = 1.f; rowf[rb] = 1.f; }
                 named_sync(1, 128);
                 const int4 fl = *reinterpret_cast<const int4 *>(flags + buf * 4);
                 const int f = fl.x | fl.y | fl.z | fl.w;
-                if (f & 2) { leave = true; break; }
+                if (f & 2) { dead = true; break; }        // the same for all four warps
                 if ((f & 1) && t > s.t0) {
                     for (int blk = 0; blk < NB; blk++)
                         for (int c0 = 0; c0 < NR; c0 += 16) {
@@ -729,8 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b_pfull);
             }
-            if (leave) break;
-            // ---- the item's result
+            // ---- the item's sums
             suma += __shfl_xor_sync(0xffffffffu, suma, 1);
             sumb += __shfl_xor_sync(0xffffffffu, sumb, 1);
             suma += __shfl_xor_sync(0xffffffffu, suma, 2);
@@ -739,51 +890,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             const size_t slot = (size_t)c * 2 + (slot1 ? 1 : 0);
             if (t4 == 0) {
                 if (s.whole) {
-                    rowf[ra] = suma == 0.f ? 0.f : 1.f / suma;
-                    rowf[rb] = sumb == 0.f ? 0.f : 1.f / sumb;
+                    rowf[ra] = suma == 0.f ? 0.f : kUnitF / suma;
+                    rowf[rb] = sumb == 0.f ? 0.f : kUnitF / sumb;
                 } else {
                     a.ml[slot * kR + ra] = make_float2(ma, suma);
                     a.ml[slot * kR + rb] = make_float2(mb, sumb);
                 }
             }
-            if (any && !dead && !mbar_wait(b_pv + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            if (any && !dead && !wait_all(b_pv + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
             tc_after();
-            named_sync(1, 128);
-            const int kv = NB * 128;
-            for (int blk = 0; blk < NB && !dead; blk++) {
-                const int col = blk * 128 + 32 * w + lane;
-                for (int c0 = 0; c0 < s.rows; c0 += 16) {
-                    float o[16];
-                    if (any) {
-                        ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = 0.f;
-                    }
-                    if (s.whole) {
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (c0 + i < s.rows) {
-                                const size_t at = (size_t)(s.row0 + c0 + i) * kv + col;
-                                const float r = o[i] * rowf[c0 + i];
-                                if (a.out_f32) ((float *)a.out)[at] = r;
-                                else ((uint16_t *)a.out)[at] = f32_to_bf16_bits(r);
-                            }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (c0 + i < s.rows) a.part[(slot * kR + c0 + i) * kv + col] = o[i];
-                    }
-                }
-            }
             tc_before();
-            named_sync(1, 128);                           // rowf is free again, O^T is read
+            named_sync(2, 384);
+            tc_after();
+            if (!dead) write_out<NB>(a, s, slot, t_o, NR, any, rowf, warp, lane);
+            tc_before();
         }
     }
     __syncthreads();
     if (warp == 12 && lane == 0) {
         // every MMA issued above has completed once this barrier flips
-        commit(b_drain);
+        commit(b_drain, 1u);
         const long long t0 = clock64();
         while (!mbar_try(b_drain, 0)) {
             if (clock64() - t0 > kSpinLimit) { k3_raise_at(K3D_ETIMEOUT, K3_SITE_CACHE4, 12, 0, (int)blockIdx.x); break; }
@@ -796,84 +922,121 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     }
 }
 
-// The pieces of each cut item, added in CTA order. Block (k, row): the k-th cut item (an item
-// is led by the first CTA boundary inside it), one of its rows; thread t has the columns
-// 4 t .. 4 t + 3 of every piece.
-__global__ void __launch_bounds__(128) k_attend4_merge(const Args a, int grid)
+// The pieces of each cut item, added in CTA order. Block (k, y, z): the k-th cut item (an item
+// is led by the first CTA boundary inside it), its row groups of four y, y + gridDim.y, ...,
+// and the z-th share of the latents. Everything that a block needs to know is loaded by its
+// threads side by side (the CTAs' info, then the pieces' maxima and sums); 512 / (kv / z)
+// threads share a latent's pieces, eight in flight each, and meet in shared memory. Few cut
+// items (one long request) take many shares, so that the pieces, 131 KB each, are read by
+// the whole card.
+constexpr int kMergeThreads = 512;
+constexpr int kMaxGrid = 512;             // CTAs of k_attend4 (one per SM)
+
+__global__ void __launch_bounds__(kMergeThreads) k_attend4_merge(const Args a, int grid, int nrg)
 {
-    __shared__ int s_c;
+    __shared__ int s_u0[kMaxGrid + 1], s_begin[kMaxGrid + 1], s_end[kMaxGrid + 1];
+    __shared__ int s_cnt[kMergeThreads / 32], s_c;
+    __shared__ float4 s_w[kMaxGrid + 1];               // a piece's weight for four rows
+    __shared__ float4 s_red[kMergeThreads / 32], s_acc[kMergeThreads];
     pdl_wait();
     pdl_trigger();
-    const int tid = threadIdx.x, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) s_c = -1;
-    __syncthreads();
-    if (tid < 32) {
-        int found = 0;
-        for (int c0 = 1; c0 < grid; c0 += 32) {
-            const int c = c0 + lane;
-            bool lead = false;
-            if (c < grid) {
-                const int4 i = a.info[2 * c];
-                lead = i.y >= 0 && i.y < i.x && a.info[2 * (c - 1)].x <= i.y;
-            }
-            const unsigned m = __ballot_sync(0xffffffffu, lead);
-            const int rank = found + __popc(m & ((1u << lane) - 1u));
-            if (lead && rank == (int)blockIdx.x) s_c = c;
-            found += __popc(m);
-        }
+    if (tid < grid) {
+        const int4 i = a.info[2 * tid];
+        s_u0[tid] = i.x;
+        s_begin[tid] = i.y;
+        s_end[tid] = i.z;
     }
+    __syncthreads();
+    const bool leads = tid >= 1 && tid < grid && s_begin[tid] >= 0 && s_begin[tid] < s_u0[tid] && s_u0[tid - 1] <= s_begin[tid];
+    const unsigned m32 = __ballot_sync(0xffffffffu, leads);
+    if (lane == 0) s_cnt[warp] = __popc(m32);
+    __syncthreads();
+    int rank = __popc(m32 & ((1u << lane) - 1u));
+    for (int i = 0; i < warp; i++) rank += s_cnt[i];
+    if (leads && rank == (int)blockIdx.x) s_c = tid;
     __syncthreads();
     const int c = s_c;
     if (c < 0) return;
-    const int4 i0 = a.info[2 * c], i1 = a.info[2 * c + 1];
-    const int r = blockIdx.y;
-    if (r >= i1.y) return;
-    const int end = i0.z;
+    const int4 i1 = a.info[2 * c + 1];                 // first row, rows
     // pieces: CTA c - 1 (its second slot unless the item begins its range), then c, c + 1, ...
-    int last = c;
-    while (last + 1 < grid && a.info[2 * (last + 1)].x < end) last++;
-    const int np = last - c + 2;
-    const size_t first = (size_t)(c - 1) * 2 + (a.info[2 * (c - 1)].x == i0.y ? 0 : 1);
+    const int np = __syncthreads_count(tid >= c && tid < grid && s_u0[tid] < s_end[c]) + 1;
+    const size_t first = (size_t)(c - 1) * 2 + (s_u0[c - 1] == s_begin[c] ? 0 : 1);
     auto slot = [&](int k) { return k == 0 ? first : (size_t)(c - 1 + k) * 2; };
-    const int kv = a.d.kv;
-    float M = __int_as_float(0xff800000);
-    for (int k = 0; k < np; k++) {
-        const float m = a.ml[slot(k) * kR + r].x;
-        M = m > M || m != m ? m : M;
-    }
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const bool on = tid * 4 < kv;
-#pragma unroll 4
-    for (int k = 0; k < np; k++) {
-        const float2 ml = a.ml[slot(k) * kR + r];
-        if (ml.x == __int_as_float(0xff800000) && ml.y == 0.f) continue;
-        const float f = exp2f(ml.x - M);
-        l += ml.y * f;
-        if (on) {
-            const float4 o = *reinterpret_cast<const float4 *>(a.part + (slot(k) * kR + r) * kv + tid * 4);
-            acc.x = fmaf(o.x, f, acc.x);
-            acc.y = fmaf(o.y, f, acc.y);
-            acc.z = fmaf(o.z, f, acc.z);
-            acc.w = fmaf(o.w, f, acc.w);
+    const float NEG = __int_as_float(0xff800000);
+    const int kv = a.d.kv, share = kv / gridDim.z, ways = kMergeThreads / share;
+    const int lat = blockIdx.z * share + tid % share, way = tid / share;
+    for (int rg = blockIdx.y; rg < nrg && rg * 4 < i1.y; rg += gridDim.y) {
+        float4 m = make_float4(NEG, NEG, NEG, NEG), l = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tid < np) {
+            const float4 *p = reinterpret_cast<const float4 *>(a.ml + slot(tid) * kR + rg * 4);
+            const float4 x = p[0], y = p[1];
+            m = make_float4(x.x, x.z, y.x, y.z);
+            l = make_float4(x.y, x.w, y.y, y.w);
         }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (on) {
-        const size_t at = (size_t)(i1.x + r) * kv + tid * 4;
-        acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-        if (a.out_f32) {
-            *reinterpret_cast<float4 *>((float *)a.out + at) = acc;
-        } else {
-            uint2 u;
-            u.x = (uint32_t)f32_to_bf16_bits(acc.x) | ((uint32_t)f32_to_bf16_bits(acc.y) << 16);
-            u.y = (uint32_t)f32_to_bf16_bits(acc.z) | ((uint32_t)f32_to_bf16_bits(acc.w) << 16);
-            *reinterpret_cast<uint2 *>((uint16_t *)a.out + at) = u;
+        auto wmax = [](float4 v) { return make_float4(warp_max(v.x), warp_max(v.y), warp_max(v.z), warp_max(v.w)); };
+        auto wsum = [](float4 v) { return make_float4(warp_sum(v.x), warp_sum(v.y), warp_sum(v.z), warp_sum(v.w)); };
+        float4 M = wmax(m);
+        if (lane == 0) s_red[warp] = M;
+        __syncthreads();
+        M = s_red[0];
+        for (int i = 1; i < kMergeThreads / 32; i++) {
+            const float4 t = s_red[i];
+            M = make_float4(fmaxf(M.x, t.x), fmaxf(M.y, t.y), fmaxf(M.z, t.z), fmaxf(M.w, t.w));
         }
+        // a piece that saw nothing has no weight
+        auto weigh = [&](float x, float top, float sum) { return x == NEG && sum == 0.f ? 0.f : exp2f(x - top); };
+        const float4 f = make_float4(weigh(m.x, M.x, l.x), weigh(m.y, M.y, l.y), weigh(m.z, M.z, l.z), weigh(m.w, M.w, l.w));
+        if (tid < np) s_w[tid] = f;
+        l = wsum(make_float4(f.x * l.x, f.y * l.y, f.z * l.z, f.w * l.w));
+        __syncthreads();
+        if (lane == 0) s_red[warp] = l;
+        __syncthreads();
+        l = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < kMergeThreads / 32; i++) {
+            const float4 t = s_red[i];
+            l.x += t.x; l.y += t.y; l.z += t.z; l.w += t.w;
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (way < ways) {
+            const float4 *src = reinterpret_cast<const float4 *>(a.part) + ((size_t)(lat >> 5) * 16 + rg) * 32 + (lat & 31);
+#pragma unroll 8
+            for (int k = way; k < np; k += ways) {
+                const float4 w = s_w[k], o = src[slot(k) * (kv / 32) * 512];
+                // without weight nothing is added, whatever the piece holds
+                acc.x = w.x != 0.f ? fmaf(o.x, w.x, acc.x) : acc.x;
+                acc.y = w.y != 0.f ? fmaf(o.y, w.y, acc.y) : acc.y;
+                acc.z = w.z != 0.f ? fmaf(o.z, w.z, acc.z) : acc.z;
+                acc.w = w.w != 0.f ? fmaf(o.w, w.w, acc.w) : acc.w;
+            }
+        }
+        if (way > 0 && way < ways) s_acc[tid] = acc;
+        __syncthreads();
+        if (way == 0) {
+            for (int i = 1; i < ways; i++) {
+                const float4 t = s_acc[i * share + tid];
+                acc.x += t.x; acc.y += t.y; acc.z += t.z; acc.w += t.w;
+            }
+            const float v[4] = {acc.x, acc.y, acc.z, acc.w}, s[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (rg * 4 + i < i1.y) {
+                    const float r = s[i] == 0.f ? 0.f : v[i] * (kUnitF / s[i]);
+                    const size_t at = (size_t)(i1.x + rg * 4 + i) * kv + lat;
+                    if (a.out_f32) ((float *)a.out)[at] = r;
+                    else ((uint16_t *)a.out)[at] = f32_to_bf16_bits(r);
+                }
+        }
+        __syncthreads();
     }
 }
 
-static int grid_size() { return sm_count() > 0 ? sm_count() : 148; }
+static int grid_size()
+{
+    const int n = sm_count() > 0 ? sm_count() : 148;
+    return n < kMaxGrid ? n : kMaxGrid;
+}
 
 static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
 
@@ -955,7 +1118,14 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
     const long long items = H <= at4::kR ? N : (long long)N * ((H + at4::kR - 1) / at4::kR);
     const int cuts = (int)(items < grid - 1 ? items : grid - 1);
     if (cuts > 0) {
-        launch_pdl(at4::k_attend4_merge, dim3(cuts, H < at4::kR ? (at4::kR / H) * H : at4::kR), dim3(128), 0, stream(), a, grid);
+        // row groups by the average rows of a request (more are looped over), and shares of the
+        // latents down to 64 while that leaves SMs without a block
+        const long long rows = ((long long)N + B - 1) / B * H;
+        const int most = (H < at4::kR ? at4::kR / H * H : at4::kR) + 3;
+        const int nrg = most / 4, y = (int)(rows < 4LL * nrg ? (rows + 3) / 4 : nrg);
+        int z = 1;
+        while (c->kv_lora / (z * 2) >= 64 && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
+        launch_pdl(at4::k_attend4_merge, dim3(cuts, y, z), dim3(at4::kMergeThreads), 0, stream(), a, grid, nrg);
         note_launch();
         K3_TRY(check_launch("mla attend4 merge"));
     }
