@@ -37,9 +37,10 @@
 //
 // ROLES (416 threads): warps 0-7 load a tile ahead into registers, widen and store it;
 // warps 8-11 do the softmax and the rescaling; these 12 load Q and write the results; warp
-// 12 issues the MMAs, tiles in pairs: S(t), S(t + 1), O(t), O(t + 1), so that the softmax of
-// one tile and the widening of the next pair run under the other's products. Every wait is
-// bounded (k3_bulk.cuh).
+// 12 issues the MMAs in the order S(t + 1), O(t). A tile is handed over in pieces of 128
+// latents: O(t) frees a piece of the buffer, the widening of tile t + 2 fills it while O(t)
+// goes on, and S(t + 2) follows it, so that the softmax of tile t + 1 has the length of O(t)
+// and S(t + 2) to run in. Every wait is bounded (k3_bulk.cuh).
 #include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"
@@ -67,6 +68,8 @@ struct Args {
     const int *table, *row_start, *kv_len;
     int max_pages, B, N, H;
     int q_f32, out_f32;
+    int per, hc;                          // tokens of an item (H <= 64), chunks of 64 heads of a token
+    float inv_h;                          // 1 / H
     float scale;
     float *part;                          // [grid][2][kv / 32][16][32][4]: latent block, row / 4, latent, row % 4
     float2 *ml;                           // [grid][2][64] (max, sum), base 2
@@ -87,7 +90,7 @@ __host__ __device__ inline Smem smem_layout(int kv, int rope)
     s.kinfo = s.p + kR * 128;             // float [2][64]: residual of each position
     s.row = s.kinfo + 2 * kT * 4;         // float [64] score factor, int [64] limit, float [64] x 2
     s.bars = s.row + 4 * kR * 4;
-    s.total = s.bars + 160 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
+    s.total = s.bars + 192 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
     return s;
 }
 
@@ -110,8 +113,7 @@ __device__ __forceinline__ Req request(const Args &a, int b)
     r.first = r0;
     r.n = n;
     r.kvl = kvl;
-    const int per = a.H <= kR ? kR / a.H : 1;
-    r.items = a.H <= kR ? (n + per - 1) / per : n * ((a.H + kR - 1) / kR);
+    r.items = a.hc > 1 ? n * a.hc : (int)((uint32_t)(n + a.per - 1) / (uint32_t)a.per);
     r.tiles = max(1, (kvl + kT - 1) / kT);
     return r;
 }
@@ -139,7 +141,7 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
         c.b++;
         c.r = request(a, c.b);
     }
-    const int item = (c.u - c.pre) / c.r.tiles;
+    const int item = (int)((uint32_t)(c.u - c.pre) / (uint32_t)c.r.tiles);
     s.b = c.b;
     s.n = c.r.n;
     s.kvl = c.r.kvl;
@@ -147,17 +149,15 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
     s.end = s.begin + c.r.tiles;
     const int first = c.r.first;
     int last;
-    if (a.H <= kR) {
-        const int per = kR / a.H;
-        s.j0 = item * per;
-        const int tok = min(per, c.r.n - s.j0);
+    if (a.hc == 1) {
+        s.j0 = item * a.per;
+        const int tok = min(a.per, c.r.n - s.j0);
         s.row0 = (first + s.j0) * a.H;
         s.rows = tok * a.H;
         last = s.j0 + tok - 1;
     } else {
-        const int hc = (a.H + kR - 1) / kR;
-        s.j0 = last = item / hc;
-        const int h0 = (item % hc) * kR;
+        s.j0 = last = (int)((uint32_t)item / (uint32_t)a.hc);
+        const int h0 = (item - s.j0 * a.hc) * kR;
         s.row0 = (first + s.j0) * a.H + h0;
         s.rows = min(kR, a.H - h0);
     }
@@ -197,23 +197,17 @@ __device__ __forceinline__ uint32_t idesc(int M, int N, int a_mn)
     return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// The whole warp runs the issue loop, so that addresses stay in uniform registers; `lead` is
-// one lane's.
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum, uint32_t lead)
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
 {
-    asm volatile("{\n\t.reg .pred p, l;\n\t"
+    asm volatile("{\n\t.reg .pred p;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "setp.ne.b32 l, %5, 0;\n\t"
-                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum), "r"(lead) : "memory");
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum) : "memory");
 }
 
-__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead)
+__device__ __forceinline__ void commit(uint32_t bar)
 {
-    asm volatile("{\n\t.reg .pred l;\n\t"
-                 "setp.ne.b32 l, %1, 0;\n\t"
-                 "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-                 :: "r"(bar), "r"(lead) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
 }
 
 __device__ __forceinline__ uint32_t elect()
@@ -297,6 +291,13 @@ __device__ __forceinline__ float unit(float e)
 // Byte `at` of row `row` in a panel of 128-byte rows, 16-byte units swizzled by the row.
 __device__ __forceinline__ uint32_t swz(int row, int unit) { return (uint32_t)(row * 128 + ((unit ^ (row & 7)) << 4)); }
 
+__device__ __forceinline__ uint2 ld_v2(const void *p)
+{
+    uint2 r;
+    asm volatile("ld.global.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p) : "memory");
+    return r;
+}
+
 // 16 bytes that no other thread reads, past L1 (a plain load: earlier work of the stream may
 // still have been writing the pool when this kernel was launched)
 __device__ __forceinline__ uint4 ld_v4(const void *p)
@@ -308,84 +309,89 @@ __device__ __forceinline__ uint4 ld_v4(const void *p)
 }
 
 // ------------------------------------------------------------------------ the widening ----
-// Thread (position, part) of a tile: 16 bytes of codes and 2 scales of every 128 latents,
-// and up to two 16-byte units of the rope key.
+// Thread (position, part) of a tile, four parts to a position: of every 128 latents the 16
+// from 16 part and the 16 from 64 + 16 part on (8 bytes of codes and a scale each), and up to
+// two 16-byte units of the rope key. The eight lanes of a store phase (two positions x four
+// parts) then hit eight different 16-byte banks.
 template <int NB>
 struct Raw {
-    uint4 code[NB];
-    uint32_t scale[NB];                   // two E4M3 bytes
+    uint2 lo[NB], hi[NB], scale[NB];      // scale: the E4M3 bytes of the 128 latents
     uint4 rope[2];
     int e;                                // exponent byte, or -1: not there
 };
 
-// The page of a position, or -1 where it is not there (past the length, or no page of the pool).
-__device__ __forceinline__ int page_at(const Args &a, int b, int pos, int kvl)
+// A thread's place in the page table, a tile at a time: the entry of the next tile is on its
+// way while this one's rows are loaded, and is checked only when it is used.
+struct Place {
+    int pos, page, in;                    // position, its page of the request, its row there
+    int entry;                            // the table's entry, -1 past the length
+};
+
+__device__ __forceinline__ void look_up(Place &p, const int *table, int kvl)
 {
-    if (pos >= kvl) return -1;
-    const int pg = a.table[(size_t)b * a.max_pages + pos / a.d.page];
-    if (pg < 0 || pg >= a.d.n_pages) {
-        k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, pg, pos);
-        return -1;
-    }
-    return pg;
+    p.entry = p.pos < kvl ? table[p.page] : -1;
 }
 
+__device__ __forceinline__ void advance(Place &p, int page)
+{
+    p.pos += kT;
+    p.in += kT;
+    while (p.in >= page) { p.in -= page; p.page++; }
+}
+
+// What is not there gets scales of 0: its latents become zeros whatever the codes are, and
+// its scores are not looked at.
 template <int NB>
-__device__ __forceinline__ void load_raw(Raw<NB> &r, const Args &a, int pg, int pos, int part)
+__device__ __forceinline__ void load_raw(Raw<NB> &r, const Args &a, const Place &p, int kvl, int part)
 {
     r.e = -1;
 #pragma unroll
-    for (int i = 0; i < NB; i++) { r.code[i] = make_uint4(0u, 0u, 0u, 0u); r.scale[i] = 0u; }
-    r.rope[0] = r.rope[1] = make_uint4(0u, 0u, 0u, 0u);
-    if (pg < 0) return;
-    const uint8_t *base = a.d.p + (size_t)pg * a.d.page_bytes;
-    const int in = pos % a.d.page;
-    const uint8_t *c = base + (size_t)in * (NB * 64) + part * 16;
-    const uint8_t *s = base + a.d.o_scale + in * (NB * 8) + part * 2;
+    for (int i = 0; i < NB; i++) r.scale[i] = make_uint2(0u, 0u);
+    if (p.pos >= kvl) return;
+    if (p.entry < 0 || p.entry >= a.d.n_pages) {          // no page of the pool: not there
+        k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, p.page, p.entry, p.pos);
+        return;
+    }
+    const uint8_t *base = a.d.p + (size_t)p.entry * a.d.page_bytes;
+    const uint8_t *c = base + p.in * (NB * 64) + part * 8;
+    const uint8_t *s = base + a.d.o_scale + p.in * (NB * 8);
 #pragma unroll
     for (int i = 0; i < NB; i++) {
-        r.code[i] = ld_v4(c + i * 64);
-        r.scale[i] = *reinterpret_cast<const uint16_t *>(s + i * 8);
+        r.lo[i] = ld_v2(c + i * 64);
+        r.hi[i] = ld_v2(c + i * 64 + 32);
+        r.scale[i] = ld_v2(s + i * 8);
     }
-    const uint8_t *rp = base + a.d.o_rope + (size_t)in * 2 * a.d.rope;
+    const uint8_t *rp = base + a.d.o_rope + p.in * 2 * a.d.rope;
     if (part < a.d.rope / 8) r.rope[0] = ld_v4(rp + part * 16);
     if (part + 4 < a.d.rope / 8) r.rope[1] = ld_v4(rp + (part + 4) * 16);
-    r.e = base[a.d.o_exp + in];
+    r.e = base[a.d.o_exp + p.in];
 }
 
-// Widens one thread's share into the tile's panels. Of the four 16-byte units that a thread
-// writes per 128 latents, parts 2 and 3 take the second pair first: the eight threads of a
-// store phase (two positions x four parts) then hit eight different 16-byte banks.
-template <int NB>
-__device__ __forceinline__ void widen(const Raw<NB> &r, uint32_t tile, int row, int part, int rope)
+__device__ __forceinline__ uint32_t unit_step(int e)
 {
-    const bool swap = part & 2;
     // 2^(e - kUnit), from 2^-14 to 1, as f16x2
-    const uint32_t up = (uint32_t)(min(max(r.e - 127 - kUnit, -kDown), 0) + 15) * 0x04000400u;
+    return (uint32_t)(min(max(e - 127 - kUnit, -kDown), 0) + 15) * 0x04000400u;
+}
+
+// This thread's 32 of 128 latents: two 16-byte units of each of two panels. at0 and at1: the
+// units' places in a panel.
+__device__ __forceinline__ void widen(uint2 lo, uint2 hi, uint2 scale, uint32_t up, uint32_t panels2, uint32_t at0,
+                                      uint32_t at1, uint32_t sel)
+{
+    uint32_t s2;                          // the two scales as f16x2
+    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(s2) : "r"(__byte_perm(scale.x, scale.y, sel)));
+    s2 = hmul2(s2, up);
+    const uint32_t f[2] = {__byte_perm(s2, s2, 0x1010), __byte_perm(s2, s2, 0x3232)};
+    const uint32_t w[4] = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-        uint32_t s2;                      // the two scales as f16x2
-        asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(s2) : "r"(r.scale[i]));
-        s2 = hmul2(s2, up);
-        const uint32_t lo = __byte_perm(s2, s2, 0x1010), hi = __byte_perm(s2, s2, 0x3232);
-        const uint32_t w[4] = {r.code[i].x, r.code[i].y, r.code[i].z, r.code[i].w};
-        const uint32_t panel = tile + (uint32_t)(2 * i + (part >> 1)) * kPanel;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t word = swap ? w[j ^ 2] : w[j];
-            const uint32_t f = ((j & 2) != 0) != swap ? hi : lo;
-            uint32_t h[4];
-            e2m1x8_to_f16x8(word, h);
-            const int unit = (part & 1) * 4 + (swap ? j ^ 2 : j);
-            sts16(panel + swz(row, unit), make_uint4(hmul2(h[0], f), hmul2(h[1], f), hmul2(h[2], f), hmul2(h[3], f)));
-        }
+    for (int j = 0; j < 4; j++) {
+        uint32_t h[4];
+        e2m1x8_to_f16x8(w[j], h);
+        const uint32_t k = f[j >> 1];
+        sts16(panels2 + (uint32_t)(j >> 1) * kPanel + ((j & 1) ? at1 : at0),
+              make_uint4(hmul2(h[0], k), hmul2(h[1], k), hmul2(h[2], k), hmul2(h[3], k)));
     }
-    const uint32_t panel = tile + (uint32_t)(2 * NB) * kPanel;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-        if (part + 4 * i < rope / 8)
-            sts16(panel + swz(row, part + 4 * i), make_uint4(hmul2(r.rope[i].x, up), hmul2(r.rope[i].y, up),
-                                                             hmul2(r.rope[i].z, up), hmul2(r.rope[i].w, up)));
 }
 
 // ------------------------------------------------------------------------------- Q ----
@@ -439,11 +445,8 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
                 for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[k]));
             }
             m = warp_max(m);
-            int e = 0;
-            if (m > 0.f && m <= 3.4028234e38f) {
-                frexpf(m, &e);
-                e = max(e, -110);
-            }
+            // m < 2^e; a row with an infinity or a NaN stays as it is
+            const int e = m <= 3.4028234e38f ? max((int)(__float_as_uint(m) >> 23) - 126, -110) : 0;
             // the sign of the scale goes into q, so that a larger product is a larger score
             const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
 #pragma unroll
@@ -466,7 +469,7 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
                 const int k = e - 14 + kUnit, k1 = k >> 1;
                 fac[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
                          __uint_as_float((uint32_t)(k - k1 + 127) << 23);
-                const int j = s.j0 + (a.H <= kR ? r / a.H : 0);
+                const int j = s.j0 + (a.hc == 1 ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
                 lim[r] = r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
             }
         }
@@ -493,7 +496,7 @@ __device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t sl
         const int blk = i / ng, c0 = (i - blk * ng) * 16;
         float o[16];
         if (any) {
-            ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+            ld16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
         } else {
 #pragma unroll
             for (int k = 0; k < 16; k++) o[k] = 0.f;
@@ -526,6 +529,56 @@ __device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t sl
     }
 }
 
+// Tensor memory columns: the CTA holds all 512, so they begin at 0. S of the two buffers, then
+// O^T, 64 columns for every 128 latents.
+constexpr uint32_t kColO = 2 * kT;
+
+// S of tile k (the k-th of this CTA) into its buffer's columns.
+template <int NB, int BUF>
+__device__ __forceinline__ bool issue_s(const Args &a, uint32_t sq, uint32_t sk, uint32_t b_kfull, uint32_t b_sfull,
+                                        volatile int *abort, int k, bool lead)
+{
+    const uint32_t pan = (uint32_t)(NB * 2 + (a.d.rope ? 1 : 0)) * kPanel;
+    const uint64_t da = desc_k(sq), db = desc_k(sk + BUF * pan);
+    constexpr uint32_t id = (1u << 4) | ((uint32_t)(kT >> 3) << 17) | ((uint32_t)(64 >> 4) << 24);
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        if (!wait_all(b_kfull + 8 * (BUF * 4 + i), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+        tc_after();
+        if (lead) {
+#pragma unroll
+            for (int p = 2 * i; p < 2 * i + 2; p++)
+#pragma unroll
+                for (int k4 = 0; k4 < 4; k4++)
+                    mma(BUF * kT, da + (p * kPanel + 32 * k4) / 16, db + (p * kPanel + 32 * k4) / 16, id, (p | k4) ? 1u : 0u);
+            if (i == NB - 1) {
+#pragma unroll
+                for (int k4 = 0; k4 < 4; k4++)
+                    if (k4 < a.d.rope / 16)
+                        mma(BUF * kT, da + (NB * 2 * kPanel + 32 * k4) / 16, db + (NB * 2 * kPanel + 32 * k4) / 16, id, 1u);
+                commit(b_sfull + 8 * BUF);
+            }
+        }
+        __syncwarp();
+    }
+    return true;
+}
+
+// O^T += V^T P^T; every 128 latents that have been used are given back.
+template <int NB, int BUF>
+__device__ __forceinline__ void issue_o(uint32_t sk, uint32_t sp, bool rope, uint32_t b_pv, uint32_t id, uint32_t accum)
+{
+    const uint32_t pan = (uint32_t)(NB * 2 + (rope ? 1 : 0)) * kPanel;
+    const uint64_t da = desc_mn(sk + BUF * pan, kPanel), db = desc_k(sp);
+#pragma unroll
+    for (int blk = 0; blk < NB; blk++) {
+#pragma unroll
+        for (int k4 = 0; k4 < kT / 16; k4++)
+            mma(kColO + blk * kR, da + (2 * blk * kPanel + 2048 * k4) / 16, db + 2 * k4, id, k4 ? 1u : accum);
+        commit(b_pv + 8 * (BUF * 4 + blk));
+    }
+}
+
 template <int NB>
 __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__ Args a)
 {
@@ -543,21 +596,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     float *rowf = reinterpret_cast<float *>(gb + L.row + 2 * kR * 4);   // rescale factors, then 1 / sum
     int *flags = reinterpret_cast<int *>(gb + L.row + 3 * kR * 4);      // [2][4]
     const uint32_t b_qfull = base + L.bars, b_qempty = b_qfull + 8;
-    const uint32_t b_kfull = b_qfull + 16, b_sfull = b_qfull + 32, b_pfull = b_qfull + 48, b_pv = b_qfull + 56;
-    const uint32_t b_drain = b_qfull + 72;
-    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 96);
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 100);
-    int *kplain = reinterpret_cast<int *>(gb + L.bars + 160);           // [2][8]
+    // of each tile buffer and 128 latents: widened (kfull), and O^T added (pv, the last of a tile
+    // standing for the tile)
+    const uint32_t b_kfull = b_qfull + 16, b_pv = b_kfull + 64, b_sfull = b_pv + 64, b_pfull = b_sfull + 16;
+    const uint32_t b_drain = b_pfull + 8;
+    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 176);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 180);
+    int *kplain = reinterpret_cast<int *>(gb + L.bars + 192);           // [2][8]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         mbar_init(b_qfull, 12);
         mbar_init(b_qempty, 1);
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 8; i++) {
             mbar_init(b_kfull + 8 * i, 8);
-            mbar_init(b_sfull + 8 * i, 1);
             mbar_init(b_pv + 8 * i, 1);
         }
+        mbar_init(b_sfull, 1);
+        mbar_init(b_sfull + 8, 1);
         mbar_init(b_pfull, 4);
         mbar_init(b_drain, 1);
         *abort = 0;
@@ -601,7 +657,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     const int U = (int)total, before = (int)min(lead, (long long)kMaxUnits);
     const int G = min((int)gridDim.x, U);
     const int c = blockIdx.x;
-    const int u0 = c < G ? (int)((long long)c * U / G) : 0, u1 = c < G ? (int)((long long)(c + 1) * U / G) : 0;
+    // the first U % G CTAs take one unit more than the others
+    const int each = G > 0 ? (int)((uint32_t)U / (uint32_t)G) : 0, more = U - each * G;
+    const int u0 = c < G ? c * each + min(c, more) : 0, u1 = c < G ? u0 + each + (c < more ? 1 : 0) : 0;
     if (u0 < u1 && u0 >= before && u0 < before + mine) {
         int pre = before;
         for (int b = rb0; b < rb1; b++) {
@@ -639,23 +697,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         a.info[2 * c + 1] = i1;
     }
     const uint32_t sq = base + L.q, sk = base + L.k, sp = base + L.p;
-    const uint32_t t_o = tmem + 128;                      // S at columns 0 and 64, O^T behind
+    constexpr uint32_t t_o = kColO;
     Seg s;
     int item = 0, g = 0;                                  // items and tiles so far (barrier phases)
 
     if (warp < 8) {
         // ------------------------------------------------------------------- widening
         const int row = tid >> 2, part = tid & 3;
+        const uint32_t at0 = swz(row, 2 * part), at1 = swz(row, 2 * part + 1);
+        const uint32_t rope0 = swz(row, part), rope1 = swz(row, part + 4);
+        const uint32_t sel = (uint32_t)(part | ((4 + part) << 4));
         bool dead = false;
         while (next_seg(a, cur, s)) {
             const bool slot1 = item > 0;                  // a later piece of this CTA
             const bool any = s.t0 < s.t1;
             Raw<NB> nx;
-            int pg = -1;
+            Place at;
+            const int *table = a.table + (size_t)s.b * a.max_pages;
+            at.pos = s.t0 * kT + row;
+            at.page = (int)((uint32_t)at.pos / (uint32_t)a.d.page);
+            at.in = at.pos - at.page * a.d.page;
             if (any) {
-                pg = page_at(a, s.b, s.t0 * kT + row, s.kvl);
-                load_raw<NB>(nx, a, pg, s.t0 * kT + row, part);
-                pg = s.t0 + 1 < s.t1 ? page_at(a, s.b, (s.t0 + 1) * kT + row, s.kvl) : -1;
+                look_up(at, table, s.kvl);
+                load_raw<NB>(nx, a, at, s.kvl, part);
+                advance(at, a.d.page);
+                look_up(at, table, s.kvl);
             }
             if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) dead = true;
             if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
@@ -666,22 +732,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             for (int t = s.t0; t < s.t1 && !dead; t++, g++) {
                 const Raw<NB> r = nx;
                 if (t + 1 < s.t1) {
-                    load_raw<NB>(nx, a, pg, (t + 1) * kT + row, part);
-                    pg = t + 2 < s.t1 ? page_at(a, s.b, (t + 2) * kT + row, s.kvl) : -1;
+                    load_raw<NB>(nx, a, at, s.kvl, part);
+                    advance(at, a.d.page);
+                    look_up(at, table, s.kvl);
                 }
                 const int buf = g & 1;
-                if (g >= 2 && !wait_all(b_pv + 8 * buf, ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
-                widen<NB>(r, sk + (uint32_t)buf * panels * kPanel, row, part, a.d.rope);
+                const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, up = unit_step(r.e);
                 // the residual; NaN for a row of NaN, minus infinity where there is none
                 const int e = r.e - 127;
                 const float res = r.e < 0 ? __int_as_float(0xff800000)
                                 : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(e - min(max(e, kUnit - kDown), kUnit));
-                if (part == 0) kinfo[buf * kT + row] = res;
                 const int plain = __all_sync(0xffffffffu, res == 0.f);
-                if (lane == 0) kplain[buf * 8 + warp] = plain;
-                async_fence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_kfull + 8 * buf);
+                // as soon as O(g - 2) has used 128 latents of the buffer, this tile's take their place
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 4 + i), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
+                    widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
+                    if (i == NB - 1) {
+                        const uint32_t pan = tile + 2 * NB * kPanel;
+                        if (part < a.d.rope / 8)
+                            sts16(pan + rope0, make_uint4(hmul2(r.rope[0].x, up), hmul2(r.rope[0].y, up), hmul2(r.rope[0].z, up), hmul2(r.rope[0].w, up)));
+                        if (part + 4 < a.d.rope / 8)
+                            sts16(pan + rope1, make_uint4(hmul2(r.rope[1].x, up), hmul2(r.rope[1].y, up), hmul2(r.rope[1].z, up), hmul2(r.rope[1].w, up)));
+                        if (part == 0) kinfo[buf * kT + row] = res;
+                        if (lane == 0) kplain[buf * 8 + warp] = plain;
+                    }
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_kfull + 8 * (buf * 4 + i));
+                }
             }
             named_sync(2, 384);                           // the item's sums are written, O^T is complete
             tc_after();
@@ -691,55 +770,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         }
     } else if (warp == 12) {
         // ------------------------------------------------------------------ MMA issuer
-        const uint32_t lead = elect();
-        const uint32_t id_s = idesc(64, kT, 0);
-        const uint32_t pan = (uint32_t)(NB * 2 + (a.d.rope ? 1 : 0)) * kPanel;
-        const int kr = a.d.rope / 16;
-        const uint32_t t_m = __shfl_sync(0xffffffffu, tmem, 0);
+        // One elected lane issues; the buffer is a constant of the code, so that the operands'
+        // addresses need no arithmetic between MMAs.
+        const bool lead = elect() != 0;
         bool stop = false;
-        auto scores = [&](int k) -> bool {                // S of the k-th tile of this CTA
-            const int buf = k & 1;
-            if (!wait_all(b_kfull + 8 * buf, (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
-            tc_after();
-            const uint32_t d = t_m + (uint32_t)(buf * kT);
-            const uint64_t da = desc_k(sq), db = desc_k(sk + (uint32_t)buf * pan);
-#pragma unroll
-            for (int p = 0; p < NB * 2; p++)
-#pragma unroll
-                for (int k4 = 0; k4 < 4; k4++)
-                    mma(d, da + (p * kPanel + 32 * k4) / 16, db + (p * kPanel + 32 * k4) / 16, id_s, (p | k4) ? 1u : 0u, lead);
-#pragma unroll
-            for (int k4 = 0; k4 < 4; k4++)
-                if (k4 < kr) mma(d, da + (NB * 2 * kPanel + 32 * k4) / 16, db + (NB * 2 * kPanel + 32 * k4) / 16, id_s, 1u, lead);
-            commit(b_sfull + 8 * buf, lead);
-            return true;
-        };
         while (!stop && next_seg(a, cur, s)) {
             if (!wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
             tc_after();
             item++;
-            const int nt = __shfl_sync(0xffffffffu, max(0, s.t1 - s.t0), 0);
-            const int NR = __shfl_sync(0xffffffffu, (s.rows + 15) & ~15, 0);      // columns of O^T
-            if (nt == 0) commit(b_qempty, lead);
-            const uint32_t id_o = idesc(128, NR, 1);
+            const int nt = max(0, s.t1 - s.t0);
+            const uint32_t id_o = idesc(128, (s.rows + 15) & ~15, 1);
+            if (nt == 0 && lead) commit(b_qempty);
             for (int i0 = 0; i0 < nt && !stop; i0 += 2) {
                 const int two = min(2, nt - i0);
-                for (int k = 0; k < two; k++) {
-                    if (!scores(g + k)) { stop = true; break; }
-                    if (i0 + k + 1 == nt) commit(b_qempty, lead);
+                for (int k = 0; k < two && !stop; k++) {
+                    stop = ((g + k) & 1) ? !issue_s<NB, 1>(a, sq, sk, b_kfull, b_sfull, abort, g + k, lead)
+                                         : !issue_s<NB, 0>(a, sq, sk, b_kfull, b_sfull, abort, g + k, lead);
+                    if (!stop && i0 + k + 1 == nt && lead) commit(b_qempty);
                 }
                 for (int k = 0; k < two && !stop; k++, g++) {
                     if (!wait_all(b_pfull, g & 1, abort, K3_SITE_CACHE4, 5, g)) { stop = true; break; }
                     tc_after();
-                    const uint64_t da = desc_mn(sk + (uint32_t)(g & 1) * pan, kPanel), db = desc_k(sp);
-                    const uint32_t acc = i0 + k ? 1u : 0u;
-#pragma unroll
-                    for (int blk = 0; blk < NB; blk++)
-#pragma unroll
-                        for (int k4 = 0; k4 < kT / 16; k4++)
-                            mma(t_m + 128 + (uint32_t)(blk * NR), da + (2 * blk * kPanel + 2048 * k4) / 16, db + 2 * k4, id_o,
-                                k4 ? 1u : acc, lead);
-                    commit(b_pv + 8 * (g & 1), lead);
+                    if (lead) {
+                        if (g & 1) issue_o<NB, 1>(sk, sp, a.d.rope != 0, b_pv, id_o, i0 + k ? 1u : 0u);
+                        else issue_o<NB, 0>(sk, sp, a.d.rope != 0, b_pv, id_o, i0 + k ? 1u : 0u);
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -767,12 +823,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
                 const int buf = g & 1;
-                if (!dead && !(wait_all(b_kfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                if (!dead && !(wait_all(b_kfull + 8 * (buf * 4 + NB - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
                                wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
                     dead = true;
                 tc_after();
                 float v[32];
-                ld_s(tmem + lanes + (uint32_t)(buf * kT), v);
+                ld_s(lanes + (uint32_t)(buf * kT), v);
                 const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
                 const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
                 const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
@@ -852,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
                 if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
                 // O(t - 1) has been added: P may be written, and the accumulator rescaled
-                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * (buf ^ 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
                 tc_after();
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -869,10 +925,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     for (int blk = 0; blk < NB; blk++)
                         for (int c0 = 0; c0 < NR; c0 += 16) {
                             float o[16];
-                            ld16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+                            ld16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
 #pragma unroll
                             for (int i = 0; i < 16; i++) o[i] *= rowf[c0 + i];
-                            st16(t_o + lanes + (uint32_t)(blk * NR + c0), o);
+                            st16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
                         }
                 }
                 if (f & 1) named_sync(1, 128);            // rowf is rewritten by the next tile
@@ -897,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     a.ml[slot * kR + rb] = make_float2(mb, sumb);
                 }
             }
-            if (any && !dead && !wait_all(b_pv + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
             tc_after();
             tc_before();
             named_sync(2, 384);
@@ -909,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     __syncthreads();
     if (warp == 12 && lane == 0) {
         // every MMA issued above has completed once this barrier flips
-        commit(b_drain, 1u);
+        commit(b_drain);
         const long long t0 = clock64();
         while (!mbar_try(b_drain, 0)) {
             if (clock64() - t0 > kSpinLimit) { k3_raise_at(K3D_ETIMEOUT, K3_SITE_CACHE4, 12, 0, (int)blockIdx.x); break; }
@@ -1102,7 +1158,8 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
     const at4::Ws w = at4::ws_layout(c->kv_lora);
     char *wb = (char *)ws;
     const at4::Args a{pool4(c, pool), q, out, table, row_start, kv_len, max_pages, B, N, H,
-                      q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, scale,
+                      q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, H <= at4::kR ? at4::kR / H : 1,
+                      (H + at4::kR - 1) / at4::kR, 1.0f / (float)H, scale,
                       (float *)(wb + w.part), (float2 *)(wb + w.ml), (int4 *)(wb + w.info)};
     const int grid = at4::grid_size();
     const size_t smem = 1024 + at4::smem_layout(c->kv_lora, c->qk_rope).total;
