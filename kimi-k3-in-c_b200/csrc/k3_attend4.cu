@@ -177,18 +177,16 @@ __device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.
 
 __device__ __forceinline__ void named_sync(int id, int n) { asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(n) : "memory"); }
 
-// SWIZZLE_128B descriptors: K-major (8-row groups 1024 B apart), and MN-major (64-element
-// blocks `lead` bytes apart, groups of 8 k 1024 B apart).
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr)
-{
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// SWIZZLE_128B descriptors, in two words: the low one has the address (16-byte units) and the
+// lead stride, the high one is a constant (groups of 8 rows, or of 8 k, 1024 B apart). K-major:
+// the lead is not used. MN-major: 64-element blocks lie `lead` bytes apart.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead)
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr, uint32_t lead)
 {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+    return ((addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
 }
 
 // kind::f16, fp32 D, fp16 A and B
@@ -197,17 +195,27 @@ __device__ __forceinline__ uint32_t idesc(int M, int N, int a_mn)
     return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accum)
+// The whole warp runs the issue loop and one lane's predicate is on the instruction. Only the
+// descriptors' low words change between MMAs: with 64-bit arithmetic on whole descriptors every
+// MMA took nine moves to uniform registers, and unrolled loops more instruction fetches than
+// MMAs' time.
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accum, uint32_t lead)
 {
-    asm volatile("{\n\t.reg .pred p;\n\t"
+    asm volatile("{\n\t.reg .pred p, l;\n\t.reg .b64 da, db;\n\t"
+                 "mov.b64 da, {%1, %6};\n\t"
+                 "mov.b64 db, {%2, %6};\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(id), "r"(accum) : "memory");
+                 "setp.ne.b32 l, %5, 0;\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 :: "r"(d), "r"(a), "r"(b), "r"(id), "r"(accum), "r"(lead), "n"(kDescHi) : "memory");
 }
 
-__device__ __forceinline__ void commit(uint32_t bar)
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+    asm volatile("{\n\t.reg .pred l;\n\t"
+                 "setp.ne.b32 l, %1, 0;\n\t"
+                 "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 :: "r"(bar), "r"(lead) : "memory");
 }
 
 __device__ __forceinline__ uint32_t elect()
@@ -220,7 +228,13 @@ __device__ __forceinline__ uint32_t elect()
 // A whole warp's bounded wait: the lanes leave together, with the same answer.
 __device__ __forceinline__ bool wait_all(uint32_t b, uint32_t parity, volatile int *abort, int site, int who, int where)
 {
-    return __all_sync(0xffffffffu, mbar_wait(b, parity, abort, site, who, where));
+    // the limit and the other roles' give-up are looked at every 32 tries only
+    bool ok = mbar_try(b, parity);
+    if (!__all_sync(0xffffffffu, ok)) {
+        for (int i = 0; i < 32 && !ok; i++) ok = mbar_try(b, parity);
+        if (!ok) ok = mbar_wait(b, parity, abort, site, who, where);
+    }
+    return __all_sync(0xffffffffu, ok);
 }
 
 #define K3_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), \
@@ -534,48 +548,48 @@ __device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t sl
 constexpr uint32_t kColO = 2 * kT;
 
 // S of tile k (the k-th of this CTA) into its buffer's columns.
-template <int NB, int BUF>
-__device__ __forceinline__ bool issue_s(const Args &a, uint32_t sq, uint32_t sk, uint32_t b_kfull, uint32_t b_sfull,
-                                        volatile int *abort, int k, bool lead)
+template <int NB>
+__device__ __forceinline__ bool issue_s(int rope, uint32_t sq, uint32_t sk, uint32_t b_kfull, uint32_t b_sfull,
+                                        volatile int *abort, int k, uint32_t lead)
 {
-    const uint32_t pan = (uint32_t)(NB * 2 + (a.d.rope ? 1 : 0)) * kPanel;
-    const uint64_t da = desc_k(sq), db = desc_k(sk + BUF * pan);
-    constexpr uint32_t id = (1u << 4) | ((uint32_t)(kT >> 3) << 17) | ((uint32_t)(64 >> 4) << 24);
-#pragma unroll
+    const int buf = k & 1;
+    uint32_t da = desc_k(sq), db = desc_k(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel);
+    const uint32_t id = idesc(64, kT, 0), d = (uint32_t)(buf * kT);
+#pragma unroll 1
     for (int i = 0; i < NB; i++) {
-        if (!wait_all(b_kfull + 8 * (BUF * 4 + i), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+        if (!wait_all(b_kfull + 8 * (buf * 4 + i), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
         tc_after();
-        if (lead) {
 #pragma unroll
-            for (int p = 2 * i; p < 2 * i + 2; p++)
+        for (int p = 0; p < 2; p++) {
 #pragma unroll
-                for (int k4 = 0; k4 < 4; k4++)
-                    mma(BUF * kT, da + (p * kPanel + 32 * k4) / 16, db + (p * kPanel + 32 * k4) / 16, id, (p | k4) ? 1u : 0u);
-            if (i == NB - 1) {
-#pragma unroll
-                for (int k4 = 0; k4 < 4; k4++)
-                    if (k4 < a.d.rope / 16)
-                        mma(BUF * kT, da + (NB * 2 * kPanel + 32 * k4) / 16, db + (NB * 2 * kPanel + 32 * k4) / 16, id, 1u);
-                commit(b_sfull + 8 * BUF);
-            }
+            for (int k4 = 0; k4 < 4; k4++) mma(d, da + 2 * k4, db + 2 * k4, id, p | k4 ? 1u : (i ? 1u : 0u), lead);
+            da += kPanel / 16;
+            db += kPanel / 16;
         }
-        __syncwarp();
     }
+#pragma unroll
+    for (int k4 = 0; k4 < 4; k4++)
+        if (k4 < rope / 16) mma(d, da + 2 * k4, db + 2 * k4, id, 1u, lead);
+    commit(b_sfull + 8 * buf, lead);
     return true;
 }
 
-// O^T += V^T P^T; every 128 latents that have been used are given back.
-template <int NB, int BUF>
-__device__ __forceinline__ void issue_o(uint32_t sk, uint32_t sp, bool rope, uint32_t b_pv, uint32_t id, uint32_t accum)
+// O^T += V^T P^T of tile k; every 128 latents that have been used are given back.
+template <int NB>
+__device__ __forceinline__ void issue_o(int rope, uint32_t sk, uint32_t sp, uint32_t b_pv, uint32_t id, int k, uint32_t accum,
+                                        uint32_t lead)
 {
-    const uint32_t pan = (uint32_t)(NB * 2 + (rope ? 1 : 0)) * kPanel;
-    const uint64_t da = desc_mn(sk + BUF * pan, kPanel), db = desc_k(sp);
-#pragma unroll
+    const int buf = k & 1;
+    uint32_t da = desc_mn(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel, kPanel), d = kColO, bar = b_pv + 32 * buf;
+    const uint32_t db = desc_k(sp);
+#pragma unroll 1
     for (int blk = 0; blk < NB; blk++) {
 #pragma unroll
-        for (int k4 = 0; k4 < kT / 16; k4++)
-            mma(kColO + blk * kR, da + (2 * blk * kPanel + 2048 * k4) / 16, db + 2 * k4, id, k4 ? 1u : accum);
-        commit(b_pv + 8 * (BUF * 4 + blk));
+        for (int k4 = 0; k4 < kT / 16; k4++) mma(d, da + 128 * k4, db + 2 * k4, id, k4 ? 1u : accum, lead);
+        commit(bar, lead);
+        da += 2 * kPanel / 16;
+        d += kR;
+        bar += 8;
     }
 }
 
@@ -770,34 +784,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         }
     } else if (warp == 12) {
         // ------------------------------------------------------------------ MMA issuer
-        // One elected lane issues; the buffer is a constant of the code, so that the operands'
-        // addresses need no arithmetic between MMAs.
-        const bool lead = elect() != 0;
-        bool stop = false;
-        while (!stop && next_seg(a, cur, s)) {
+        const uint32_t lead = elect();
+        for (;;) {
+            const bool have = next_seg(a, cur, s);
+            if (!__any_sync(0xffffffffu, have)) break;
             if (!wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
             tc_after();
             item++;
-            const int nt = max(0, s.t1 - s.t0);
-            const uint32_t id_o = idesc(128, (s.rows + 15) & ~15, 1);
-            if (nt == 0 && lead) commit(b_qempty);
-            for (int i0 = 0; i0 < nt && !stop; i0 += 2) {
-                const int two = min(2, nt - i0);
-                for (int k = 0; k < two && !stop; k++) {
-                    stop = ((g + k) & 1) ? !issue_s<NB, 1>(a, sq, sk, b_kfull, b_sfull, abort, g + k, lead)
-                                         : !issue_s<NB, 0>(a, sq, sk, b_kfull, b_sfull, abort, g + k, lead);
-                    if (!stop && i0 + k + 1 == nt && lead) commit(b_qempty);
-                }
-                for (int k = 0; k < two && !stop; k++, g++) {
-                    if (!wait_all(b_pfull, g & 1, abort, K3_SITE_CACHE4, 5, g)) { stop = true; break; }
+            const int nt = __reduce_max_sync(0xffffffffu, max(0, s.t1 - s.t0));
+            const uint32_t id_o = idesc(128, __reduce_max_sync(0xffffffffu, (s.rows + 15) & ~15), 1);
+            if (nt == 0) commit(b_qempty, lead);
+            bool stop = false;
+            for (int i = 0; i < nt && !stop; i++) {
+                // S of tile i and, behind every second one and the last, O of the pair
+                const int k = g + i;
+                stop = !issue_s<NB>(a.d.rope, sq, sk, b_kfull, b_sfull, abort, k, lead);
+                if (stop) break;
+                if (i + 1 == nt) commit(b_qempty, lead);
+                else if (!(i & 1)) continue;
+                for (int j = i & ~1; j <= i; j++) {
+                    if (!wait_all(b_pfull, (g + j) & 1, abort, K3_SITE_CACHE4, 5, g + j)) { stop = true; break; }
                     tc_after();
-                    if (lead) {
-                        if (g & 1) issue_o<NB, 1>(sk, sp, a.d.rope != 0, b_pv, id_o, i0 + k ? 1u : 0u);
-                        else issue_o<NB, 0>(sk, sp, a.d.rope != 0, b_pv, id_o, i0 + k ? 1u : 0u);
-                    }
-                    __syncwarp();
+                    issue_o<NB>(a.d.rope, sk, sp, b_pv, id_o, g + j, j ? 1u : 0u, lead);
                 }
             }
+            if (stop) break;
+            g += nt;
         }
         __syncwarp();
     } else {
@@ -965,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     __syncthreads();
     if (warp == 12 && lane == 0) {
         // every MMA issued above has completed once this barrier flips
-        commit(b_drain);
+        commit(b_drain, 1u);
         const long long t0 = clock64();
         while (!mbar_try(b_drain, 0)) {
             if (clock64() - t0 > kSpinLimit) { k3_raise_at(K3D_ETIMEOUT, K3_SITE_CACHE4, 12, 0, (int)blockIdx.x); break; }
