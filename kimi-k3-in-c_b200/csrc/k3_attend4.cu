@@ -55,9 +55,6 @@ constexpr int kR = 64;                    // rows per item
 constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
 constexpr int kThreads = 416;
 constexpr int kMaxUnits = 1 << 30;
-// Tensor memory columns: the CTA holds all 512, so they begin at 0. S of the two buffers, then
-// O^T, 64 columns for every 128 latents.
-constexpr uint32_t kColO = 2 * kT;
 constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
 constexpr float kStep = 8.f;              // m moves when a tile passes it by this
 constexpr int kUnit = -2;                 // the fp16 operand is in units of 2^kUnit
@@ -412,161 +409,143 @@ __device__ __forceinline__ void widen(uint2 lo, uint2 hi, uint2 scale, uint32_t 
 }
 
 // ------------------------------------------------------------------------------- Q ----
-// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the row's largest value in
-// [2^13, 2^14)), the score factor and the number of positions the row sees. Rows behind the
-// last are zeros that see everything: they cost no case of their own. The next row is on
-// its way while one is converted. The loop is rolled and both roles run the same copy: the code runs
-// once per item, and every 128 bytes of it are fetched from L2 first (unrolled, and once for
-// each role, it took 8000 cycles, more than a tile).
-struct QJob {
-    const char *src;                      // the item's first row
-    int rows, chunks;                     // rows, and 8-value chunks of a row
-    int f32, one_head_chunk;
-    float scale, inv_h;
-    int seen0;                            // positions that the item's first token sees
-    uint32_t dst;
-    float *fac;
-    int *lim;
-};
-
-__device__ __forceinline__ void load_q(const QJob j, int warp, int lane)
+// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the
+// row's largest value in [2^13, 2^14)), the score factor and the number of positions the row
+// sees. Rows behind the last are zeros that see everything: they cost no case of their own.
+template <bool F32>
+__device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
 {
-    struct Row { uint4 v[3], w[3]; };
-    const uint32_t esz = j.f32 ? 4 : 2;
-    auto fetch = [&](Row &t, int r) {
-        const char *p = j.src + (size_t)r * j.chunks * 8 * esz + lane * 8 * esz;
+    constexpr int RB = F32 ? 1 : 3;                       // rows in flight (36 registers or 24)
+    const int W = a.d.kv + a.d.rope, chunks = W / 8;
+    for (int r0 = warp; r0 < kR; r0 += 12 * RB) {
+        uint4 raw[RB][3][F32 ? 2 : 1];
 #pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const bool on = r < j.rows && lane + 32 * c < j.chunks;
-            t.v[c] = t.w[c] = make_uint4(0u, 0u, 0u, 0u);
-            if (on) t.v[c] = *reinterpret_cast<const uint4 *>(p + c * 256 * esz);
-            if (on && j.f32) t.w[c] = *reinterpret_cast<const uint4 *>(p + c * 256 * esz + 16);
-        }
-    };
-    Row cur;
-    fetch(cur, warp);
-#pragma unroll 1
-    for (int r = warp; r < kR; r += 12) {
-        Row next;
-        fetch(next, r + 12);
-        float v[3][8];
-        float m = 0.f;
+        for (int i = 0; i < RB; i++) {
+            const int r = r0 + 12 * i;
+            const size_t at = (size_t)(s.row0 + r) * W;
 #pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const uint32_t u[8] = {cur.v[c].x, cur.v[c].y, cur.v[c].z, cur.v[c].w, cur.w[c].x, cur.w[c].y, cur.w[c].z, cur.w[c].w};
+            for (int c = 0; c < 3; c++) {
+                const int ch = lane + 32 * c;
+                const uint4 *p = reinterpret_cast<const uint4 *>((const char *)a.q + (at + ch * 8) * (F32 ? 4 : 2));
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const uint32_t h = k & 1 ? u[k / 2] & 0xffff0000u : u[k / 2] << 16;
-                v[c][k] = __uint_as_float(j.f32 ? u[k] : h);
-                m = fmaxf(m, fabsf(v[c][k]));
+                for (int k = 0; k < (F32 ? 2 : 1); k++)
+                    raw[i][c][k] = ch < chunks && r < s.rows ? p[k] : make_uint4(0u, 0u, 0u, 0u);
             }
         }
-        m = warp_max(m);
-        // m < 2^e; a row with an infinity or a NaN stays as it is
-        const int e = m <= 3.4028234e38f ? max((int)(__float_as_uint(m) >> 23) - 126, -110) : 0;
-        // the sign of the scale goes into q, so that a larger product is a larger score
-        const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), j.scale);
 #pragma unroll
-        for (int c = 0; c < 3; c++) {
-            const int ch = lane + 32 * c;
-            uint32_t h[4];
+        for (int i = 0; i < RB; i++) {
+            const int r = r0 + 12 * i;
+            if (r >= kR) break;
+            auto value = [&](int c, float v[8]) {
+                const uint4 x = raw[i][c][0], y = raw[i][c][F32 ? 1 : 0];
+                const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                if (F32) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const __half2 t = __floats2half2_rn(v[c][2 * k] * up, v[c][2 * k + 1] * up);
-                h[k] = *reinterpret_cast<const uint32_t *>(&t);
+                    for (int k = 0; k < 8; k++) v[k] = __uint_as_float(u[k]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        v[2 * k] = __uint_as_float(u[k] << 16);
+                        v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
+                    }
+                }
+            };
+            float m = 0.f;
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                float v[8];
+                value(c, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[k]));
             }
-            if (ch < j.chunks) sts16(j.dst + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
+            m = warp_max(m);
+            // m < 2^e; a row with an infinity or a NaN stays as it is
+            const int e = m <= 3.4028234e38f ? max((int)(__float_as_uint(m) >> 23) - 126, -110) : 0;
+            // the sign of the scale goes into q, so that a larger product is a larger score
+            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
+#pragma unroll
+            for (int c = 0; c < 3; c++) {
+                const int ch = lane + 32 * c;
+                if (ch < chunks) {
+                    float v[8];
+                    value(c, v);
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const __half2 t = __floats2half2_rn(v[2 * k] * up, v[2 * k + 1] * up);
+                        h[k] = *reinterpret_cast<const uint32_t *>(&t);
+                    }
+                    sts16(sq + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
+                }
+            }
+            if (lane == 0) {
+                // |scale| log2(e) 2^(e - 14 + kUnit), the power in two factors (it may be below -126)
+                const int k = e - 14 + kUnit, k1 = k >> 1;
+                fac[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
+                         __uint_as_float((uint32_t)(k - k1 + 127) << 23);
+                const int j = s.j0 + (a.hc == 1 ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
+                lim[r] = r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
+            }
         }
-        if (lane == 0) {
-            // |scale| log2(e) 2^(e - 14 + kUnit), the power in two factors (it may be below -126)
-            const int k = e - 14 + kUnit, k1 = k >> 1;
-            j.fac[r] = fabsf(j.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
-                       __uint_as_float((uint32_t)(k - k1 + 127) << 23);
-            const int tok = j.one_head_chunk ? (int)(((float)r + 0.5f) * j.inv_h) : 0;
-            j.lim[r] = r < j.rows ? max(0, j.seen0 + tok) : 0x7fffffff;
-        }
-        cur = next;
     }
 }
 
-__device__ __forceinline__ QJob q_job(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim)
+__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
 {
-    const int W = a.d.kv + a.d.rope;
-    QJob j;
-    j.src = (const char *)a.q + (size_t)s.row0 * W * (a.q_f32 ? 4 : 2);
-    j.rows = s.rows; j.chunks = W / 8;
-    j.f32 = a.q_f32; j.one_head_chunk = a.hc == 1;
-    j.scale = a.scale; j.inv_h = a.inv_h;
-    j.seen0 = s.kvl - s.n + s.j0 + 1;
-    j.dst = sq; j.fac = fac; j.lim = lim;
-    return j;
+    if (a.q_f32) load_q_rows<true>(a, s, sq, fac, lim, warp, lane);
+    else load_q_rows<false>(a, s, sq, fac, lim, warp, lane);
 }
 
 // This warp's third of an item's result: the 16-row groups sub, sub + 3, ... of its quarter of
 // the lanes (latents). A whole item: neighbouring lanes trade halves, so that each writes a
 // pair of latents of eight rows. A piece: as it lies, four rows to a 16-byte store.
-struct OJob {
-    char *dst;                            // the item's first row, or the piece
-    int rows, whole, any, f32;
-    const float *rowf;
-};
-
 template <int NB>
-__device__ __forceinline__ void write_out(const OJob j, int warp, int lane)
+__device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t slot, uint32_t t_o, int NR, bool any,
+                                          const float *rowf, int warp, int lane)
 {
-    const int q = warp & 3, ng = (j.rows + 15) >> 4;
+    const int q = warp & 3, sub = warp >> 2, ng = NR / 16;
     const uint32_t lanes = (uint32_t)(32 * q) << 16;
     constexpr int kv = NB * 128;
-    int blk = 0, grp = warp >> 2;
-#pragma unroll 1
-    for (; ; grp += 3) {
-        while (grp >= ng) { grp -= ng; blk++; }
-        if (blk >= NB) break;
-        const int c0 = grp * 16;
+    for (int i = sub; i < NB * ng; i += 3) {
+        const int blk = i / ng, c0 = (i - blk * ng) * 16;
         float o[16];
-        if (j.any) {
-            ld16(kColO + lanes + (uint32_t)(blk * kR + c0), o);
+        if (any) {
+            ld16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
         } else {
 #pragma unroll
             for (int k = 0; k < 16; k++) o[k] = 0.f;
         }
-        if (j.whole) {
-            const int col = blk * 128 + 32 * q + (lane & ~1), r0 = c0 + (lane & 1) * 8;
-            const uint32_t esz = j.f32 ? 4 : 2;
-            char *p = j.dst + ((size_t)r0 * kv + col) * esz;
+        if (s.whole) {
+            const int col = blk * 128 + 32 * q + (lane & ~1), up = (lane & 1) * 8;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float give = (lane & 1) ? o[k] : o[k + 8];
                 const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-                const float f = j.rowf[r0 + k];
-                const float x = ((lane & 1) ? got : o[k]) * f, y = ((lane & 1) ? o[k + 8] : got) * f;
-                if (r0 + k < j.rows) {
-                    if (j.f32)
-                        *reinterpret_cast<float2 *>(p) = make_float2(x, y);
-                    else
-                        *reinterpret_cast<uint32_t *>(p) = (uint32_t)f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16);
+                const int r = c0 + k + up;
+                if (r < s.rows) {
+                    const float f = rowf[r];
+                    const float x = ((lane & 1) ? got : o[k]) * f, y = ((lane & 1) ? o[k + 8] : got) * f;
+                    const size_t at = (size_t)(s.row0 + r) * kv + col;
+                    if (a.out_f32) {
+                        *reinterpret_cast<float2 *>((float *)a.out + at) = make_float2(x, y);
+                    } else {
+                        *reinterpret_cast<uint32_t *>((uint16_t *)a.out + at) =
+                            (uint32_t)f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16);
+                    }
                 }
-                p += kv * esz;
             }
         } else {
-            float4 *dst = reinterpret_cast<float4 *>(j.dst) + ((blk * 4 + q) * 16 + c0 / 4) * 32 + lane;
+            float4 *dst = reinterpret_cast<float4 *>(a.part) + ((slot * (NB * 4) + blk * 4 + q) * 16 + c0 / 4) * 32 + lane;
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                if (c0 + 4 * k < j.rows) dst[k * 32] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                if (c0 + 4 * k < s.rows) dst[k * 32] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
     }
 }
 
-template <int NB>
-__device__ __forceinline__ OJob o_job(const Args &a, const Seg &s, size_t slot, bool any, const float *rowf)
-{
-    constexpr int kv = NB * 128;
-    OJob j;
-    j.dst = s.whole ? (char *)a.out + (size_t)s.row0 * kv * (a.out_f32 ? 4 : 2) : (char *)(a.part + slot * kR * kv);
-    j.rows = s.rows; j.whole = s.whole; j.any = any; j.f32 = a.out_f32;
-    j.rowf = rowf;
-    return j;
-}
+// Tensor memory columns: the CTA holds all 512, so they begin at 0. S of the two buffers, then
+// O^T, 64 columns for every 128 latents.
+constexpr uint32_t kColO = 2 * kT;
 
 // S of tile k (the k-th of this CTA) into its buffer's columns.
 template <int NB>
@@ -736,20 +715,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     Seg s;
     int item = 0, g = 0;                                  // items and tiles so far (barrier phases)
 
-    if (warp < 12) {
-        // widening (warps 0-7)
+    if (warp < 8) {
+        // ------------------------------------------------------------------- widening
         const int row = tid >> 2, part = tid & 3;
         const uint32_t at0 = swz(row, 2 * part), at1 = swz(row, 2 * part + 1);
         const uint32_t rope0 = swz(row, part), rope1 = swz(row, part + 4);
         const uint32_t sel = (uint32_t)(part | ((4 + part) << 4));
-        // softmax, rescaling (warps 8-11)
-        const int w = warp - 8, gr = lane >> 2, t4 = lane & 3;
-        const int ra = 16 * w + gr, rb = ra + 8;          // this thread's rows
-        const float NEG = __int_as_float(0xff800000);
-        const uint32_t lanes = (uint32_t)(32 * w) << 16;
         bool dead = false;
         while (next_seg(a, cur, s)) {
-            const size_t slot = (size_t)c * 2 + (item > 0 ? 1 : 0);           // a later piece of this CTA: the second
+            const bool slot1 = item > 0;                  // a later piece of this CTA
             const bool any = s.t0 < s.t1;
             Raw<NB> nx;
             Place at;
@@ -757,201 +731,58 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             at.pos = s.t0 * kT + row;
             at.page = (int)((uint32_t)at.pos / (uint32_t)a.d.page);
             at.in = at.pos - at.page * a.d.page;
-            if (any && warp < 8) {
+            if (any) {
                 look_up(at, table, s.kvl);
                 load_raw<NB>(nx, a, at, s.kvl, part);
                 advance(at, a.d.page);
                 look_up(at, table, s.kvl);
             }
             if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) dead = true;
-            if (!dead) load_q(q_job(a, s, sq, fac, lim), warp, lane);
+            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
             async_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_qfull);
-            if (warp < 8) {
-                // --------------------------------------------------------------- widening
-                for (int t = s.t0; t < s.t1 && !dead; t++, g++) {
-                    const Raw<NB> r = nx;
-                    if (t + 1 < s.t1) {
-                        load_raw<NB>(nx, a, at, s.kvl, part);
-                        advance(at, a.d.page);
-                        look_up(at, table, s.kvl);
-                    }
-                    const int buf = g & 1;
-                    const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, up = unit_step(r.e);
-                    // the residual; NaN for a row of NaN, minus infinity where there is none
-                    const int e = r.e - 127;
-                    const float res = r.e < 0 ? __int_as_float(0xff800000)
-                                    : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(e - min(max(e, kUnit - kDown), kUnit));
-                    const int plain = __all_sync(0xffffffffu, res == 0.f);
-                    // as soon as O(g - 2) has used 128 latents of the buffer, this tile's take their place
-#pragma unroll
-                    for (int i = 0; i < NB; i++) {
-                        if (g >= 2 && !wait_all(b_pv + 8 * (buf * 4 + i), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
-                        widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
-                        if (i == NB - 1) {
-                            const uint32_t pan = tile + 2 * NB * kPanel;
-                            if (part < a.d.rope / 8)
-                                sts16(pan + rope0, make_uint4(hmul2(r.rope[0].x, up), hmul2(r.rope[0].y, up), hmul2(r.rope[0].z, up), hmul2(r.rope[0].w, up)));
-                            if (part + 4 < a.d.rope / 8)
-                                sts16(pan + rope1, make_uint4(hmul2(r.rope[1].x, up), hmul2(r.rope[1].y, up), hmul2(r.rope[1].z, up), hmul2(r.rope[1].w, up)));
-                            if (part == 0) kinfo[buf * kT + row] = res;
-                            if (lane == 0) kplain[buf * 8 + warp] = plain;
-                        }
-                        async_fence();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(b_kfull + 8 * (buf * 4 + i));
-                    }
-                }
-            } else {
-                // ------------------------------------------------------ softmax, rescale
-                if (!dead && !wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
-                const int NR = (s.rows + 15) & ~15;
-                const float fa = fac[ra], fb = fac[rb];
-                const int la = lim[ra], lb = lim[rb];
-                const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
-                float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
-                for (int t = s.t0; t < s.t1; t++, g++) {
-                    const int buf = g & 1;
-                    if (!dead && !(wait_all(b_kfull + 8 * (buf * 4 + NB - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
-                                   wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
-                        dead = true;
-                    tc_after();
-                    float v[32];
-                    ld_s(lanes + (uint32_t)(buf * kT), v);
-                    const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
-                    const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
-                    const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
-                    float ca = 1.f, cb = 1.f;
-                    // moves the references to a tile's maxima; a row's accumulator changes only if
-                    // it held something
-                    auto move = [&](float xa, float xb) {
-                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
-                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
-                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
-                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
-                        if (ma == NEG) ma = xa;
-                        else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
-                        if (mb == NEG) mb = xb;
-                        else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
-                    };
-                    uint32_t pa[8], pb[8];
-                    if (plain) {
-                        // every row sees the whole tile, no residuals: the product's maximum is the
-                        // score's, and the sum adds what P is rounded from
-                        float xa = fmaxf(v[0], v[1]), xb = fmaxf(v[2], v[3]);
-#pragma unroll
-                        for (int i = 1; i < 8; i++) {
-                            xa = fmaxf(xa, fmaxf(v[4 * i], v[4 * i + 1]));
-                            xb = fmaxf(xb, fmaxf(v[4 * i + 2], v[4 * i + 3]));
-                        }
-                        move(xa * fa, xb * fb);
-                        const float na = kLift - (ma == NEG ? 0.f : ma), nb = kLift - (mb == NEG ? 0.f : mb);
-                        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float p0 = ex2(fmaf(v[4 * i], fa, na)), p1 = ex2(fmaf(v[4 * i + 1], fa, na));
-                            const float p2 = ex2(fmaf(v[4 * i + 2], fb, nb)), p3 = ex2(fmaf(v[4 * i + 3], fb, nb));
-                            s0 += p0; s1 += p1; s2 += p2; s3 += p3;
-                            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                            pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
-                            pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
-                        }
-                        suma += s0 + s1;
-                        sumb += s2 + s3;
-                    } else {
-                        const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
-                        float xa = NEG, xb = NEG;
-                        float kr[16];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float2 k = ki[4 * i + t4];  // residuals of two neighbouring positions
-                            const float u0 = unit(k.x), u1 = unit(k.y);
-                            const int pos = t * kT + 8 * i + 2 * t4;
-                            kr[2 * i] = k.x;
-                            kr[2 * i + 1] = k.y;
-                            const bool h0 = k.x != NEG, h1 = k.y != NEG;
-                            v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
-                            v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
-                            v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
-                            v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
-                            xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
-                            xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
-                        }
-                        move(xa, xb);
-                        const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float r0 = kr[2 * i], r1 = kr[2 * i + 1];
-                            suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
-                            sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
-                            // a masked position is minus infinity whatever its residual is
-                            const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + r0 - na);
-                            const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + r1 - na);
-                            const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + r0 - nb);
-                            const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + r1 - nb);
-                            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                            pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
-                            pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
-                        }
-                    }
-                    const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
-                    if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
-                    // O(t - 1) has been added: P may be written, and the accumulator rescaled
-                    if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
-                    tc_after();
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
-                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
-                    }
-                    if (moved && t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
-                    if (!moved && t4 == 0) { rowf[ra] = 1.f; rowf[rb] = 1.f; }
-                    named_sync(1, 128);
-                    const int4 fl = *reinterpret_cast<const int4 *>(flags + buf * 4);
-                    const int f = fl.x | fl.y | fl.z | fl.w;
-                    if (f & 2) { dead = true; break; }        // the same for all four warps
-                    if ((f & 1) && t > s.t0) {
-                        for (int blk = 0; blk < NB; blk++)
-                            for (int c0 = 0; c0 < NR; c0 += 16) {
-                                float o[16];
-                                ld16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
-#pragma unroll
-                                for (int i = 0; i < 16; i++) o[i] *= rowf[c0 + i];
-                                st16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
-                            }
-                    }
-                    if (f & 1) named_sync(1, 128);            // rowf is rewritten by the next tile
-                    async_fence();
-                    tc_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(b_pfull);
-                }
-                // ---- the item's sums
-                suma += __shfl_xor_sync(0xffffffffu, suma, 1);
-                sumb += __shfl_xor_sync(0xffffffffu, sumb, 1);
-                suma += __shfl_xor_sync(0xffffffffu, suma, 2);
-                sumb += __shfl_xor_sync(0xffffffffu, sumb, 2);
-                if (t4 == 0) {
-                    if (s.whole) {
-                        rowf[ra] = suma == 0.f ? 0.f : kUnitF / suma;
-                        rowf[rb] = sumb == 0.f ? 0.f : kUnitF / sumb;
-                    } else {
-                        a.ml[slot * kR + ra] = make_float2(ma, suma);
-                        a.ml[slot * kR + rb] = make_float2(mb, sumb);
-                    }
-                }
-                if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
-                tc_after();
-                tc_before();
-            }
             item++;
+            for (int t = s.t0; t < s.t1 && !dead; t++, g++) {
+                const Raw<NB> r = nx;
+                if (t + 1 < s.t1) {
+                    load_raw<NB>(nx, a, at, s.kvl, part);
+                    advance(at, a.d.page);
+                    look_up(at, table, s.kvl);
+                }
+                const int buf = g & 1;
+                const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, up = unit_step(r.e);
+                // the residual; NaN for a row of NaN, minus infinity where there is none
+                const int e = r.e - 127;
+                const float res = r.e < 0 ? __int_as_float(0xff800000)
+                                : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(e - min(max(e, kUnit - kDown), kUnit));
+                const int plain = __all_sync(0xffffffffu, res == 0.f);
+                // as soon as O(g - 2) has used 128 latents of the buffer, this tile's take their place
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 4 + i), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
+                    widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
+                    if (i == NB - 1) {
+                        const uint32_t pan = tile + 2 * NB * kPanel;
+                        if (part < a.d.rope / 8)
+                            sts16(pan + rope0, make_uint4(hmul2(r.rope[0].x, up), hmul2(r.rope[0].y, up), hmul2(r.rope[0].z, up), hmul2(r.rope[0].w, up)));
+                        if (part + 4 < a.d.rope / 8)
+                            sts16(pan + rope1, make_uint4(hmul2(r.rope[1].x, up), hmul2(r.rope[1].y, up), hmul2(r.rope[1].z, up), hmul2(r.rope[1].w, up)));
+                        if (part == 0) kinfo[buf * kT + row] = res;
+                        if (lane == 0) kplain[buf * 8 + warp] = plain;
+                    }
+                    async_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_kfull + 8 * (buf * 4 + i));
+                }
+            }
             named_sync(2, 384);                           // the item's sums are written, O^T is complete
             tc_after();
-            if (!dead) write_out<NB>(o_job<NB>(a, s, slot, any, rowf), warp, lane);
+            if (!dead)
+                write_out<NB>(a, s, (size_t)c * 2 + (slot1 ? 1 : 0), t_o, (s.rows + 15) & ~15, any, rowf, warp, lane);
             tc_before();
         }
-    } else {
+    } else if (warp == 12) {
         // ------------------------------------------------------------------ MMA issuer
         const uint32_t lead = elect();
         for (;;) {
@@ -981,6 +812,167 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             g += nt;
         }
         __syncwarp();
+    } else {
+        // --------------------------------------------------- softmax, rescale, results
+        const int w = warp - 8, gr = lane >> 2, t4 = lane & 3;
+        const int ra = 16 * w + gr, rb = ra + 8;          // this thread's rows
+        const float NEG = __int_as_float(0xff800000);
+        const uint32_t lanes = (uint32_t)(32 * w) << 16;
+        bool dead = false;
+        while (next_seg(a, cur, s)) {
+            const bool slot1 = item > 0;
+            if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 6, item)) dead = true;
+            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_qfull);
+            if (!dead && !wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
+            item++;
+            const int NR = (s.rows + 15) & ~15;
+            const float fa = fac[ra], fb = fac[rb];
+            const int la = lim[ra], lb = lim[rb];
+            const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
+            float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
+            for (int t = s.t0; t < s.t1; t++, g++) {
+                const int buf = g & 1;
+                if (!dead && !(wait_all(b_kfull + 8 * (buf * 4 + NB - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                               wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
+                    dead = true;
+                tc_after();
+                float v[32];
+                ld_s(lanes + (uint32_t)(buf * kT), v);
+                const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
+                const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
+                const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
+                float ca = 1.f, cb = 1.f;
+                // moves the references to a tile's maxima; a row's accumulator changes only if
+                // it held something
+                auto move = [&](float xa, float xb) {
+                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
+                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
+                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
+                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
+                    if (ma == NEG) ma = xa;
+                    else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
+                    if (mb == NEG) mb = xb;
+                    else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
+                };
+                uint32_t pa[8], pb[8];
+                if (plain) {
+                    // every row sees the whole tile, no residuals: the product's maximum is the
+                    // score's, and the sum adds what P is rounded from
+                    float xa = fmaxf(v[0], v[1]), xb = fmaxf(v[2], v[3]);
+#pragma unroll
+                    for (int i = 1; i < 8; i++) {
+                        xa = fmaxf(xa, fmaxf(v[4 * i], v[4 * i + 1]));
+                        xb = fmaxf(xb, fmaxf(v[4 * i + 2], v[4 * i + 3]));
+                    }
+                    move(xa * fa, xb * fb);
+                    const float na = kLift - (ma == NEG ? 0.f : ma), nb = kLift - (mb == NEG ? 0.f : mb);
+                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float p0 = ex2(fmaf(v[4 * i], fa, na)), p1 = ex2(fmaf(v[4 * i + 1], fa, na));
+                        const float p2 = ex2(fmaf(v[4 * i + 2], fb, nb)), p3 = ex2(fmaf(v[4 * i + 3], fb, nb));
+                        s0 += p0; s1 += p1; s2 += p2; s3 += p3;
+                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                    }
+                    suma += s0 + s1;
+                    sumb += s2 + s3;
+                } else {
+                    const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
+                    float xa = NEG, xb = NEG;
+                    float kr[16];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float2 k = ki[4 * i + t4];  // residuals of two neighbouring positions
+                        const float u0 = unit(k.x), u1 = unit(k.y);
+                        const int pos = t * kT + 8 * i + 2 * t4;
+                        kr[2 * i] = k.x;
+                        kr[2 * i + 1] = k.y;
+                        const bool h0 = k.x != NEG, h1 = k.y != NEG;
+                        v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
+                        v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
+                        v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
+                        v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
+                        xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
+                        xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
+                    }
+                    move(xa, xb);
+                    const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float r0 = kr[2 * i], r1 = kr[2 * i + 1];
+                        suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
+                        sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
+                        // a masked position is minus infinity whatever its residual is
+                        const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + r0 - na);
+                        const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + r1 - na);
+                        const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + r0 - nb);
+                        const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + r1 - nb);
+                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                    }
+                }
+                const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
+                if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
+                // O(t - 1) has been added: P may be written, and the accumulator rescaled
+                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                tc_after();
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
+                }
+                if (moved && t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
+                if (!moved && t4 == 0) { rowf[ra] = 1.f; rowf[rb] = 1.f; }
+                named_sync(1, 128);
+                const int4 fl = *reinterpret_cast<const int4 *>(flags + buf * 4);
+                const int f = fl.x | fl.y | fl.z | fl.w;
+                if (f & 2) { dead = true; break; }        // the same for all four warps
+                if ((f & 1) && t > s.t0) {
+                    for (int blk = 0; blk < NB; blk++)
+                        for (int c0 = 0; c0 < NR; c0 += 16) {
+                            float o[16];
+                            ld16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] *= rowf[c0 + i];
+                            st16(t_o + lanes + (uint32_t)(blk * kR + c0), o);
+                        }
+                }
+                if (f & 1) named_sync(1, 128);            // rowf is rewritten by the next tile
+                async_fence();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_pfull);
+            }
+            // ---- the item's sums
+            suma += __shfl_xor_sync(0xffffffffu, suma, 1);
+            sumb += __shfl_xor_sync(0xffffffffu, sumb, 1);
+            suma += __shfl_xor_sync(0xffffffffu, suma, 2);
+            sumb += __shfl_xor_sync(0xffffffffu, sumb, 2);
+            const bool any = s.t0 < s.t1;
+            const size_t slot = (size_t)c * 2 + (slot1 ? 1 : 0);
+            if (t4 == 0) {
+                if (s.whole) {
+                    rowf[ra] = suma == 0.f ? 0.f : kUnitF / suma;
+                    rowf[rb] = sumb == 0.f ? 0.f : kUnitF / sumb;
+                } else {
+                    a.ml[slot * kR + ra] = make_float2(ma, suma);
+                    a.ml[slot * kR + rb] = make_float2(mb, sumb);
+                }
+            }
+            if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            tc_after();
+            tc_before();
+            named_sync(2, 384);
+            tc_after();
+            if (!dead) write_out<NB>(a, s, slot, t_o, NR, any, rowf, warp, lane);
+            tc_before();
+        }
     }
     __syncthreads();
     if (warp == 12 && lane == 0) {
