@@ -53,7 +53,7 @@ using namespace bulk;
 constexpr int kT = 64;                    // positions per tile
 constexpr int kR = 64;                    // rows per item
 constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
-constexpr int kThreads = 416;
+constexpr int kThreads = 448;
 constexpr int kMaxUnits = 1 << 30;
 constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
 constexpr float kStep = 8.f;              // m moves when a tile passes it by this
@@ -90,7 +90,7 @@ __host__ __device__ inline Smem smem_layout(int kv, int rope)
     s.kinfo = s.p + kR * 128;             // float [2][64]: residual of each position
     s.row = s.kinfo + 2 * kT * 4;         // float [64] score factor, int [64] limit, float [64] x 2
     s.bars = s.row + 4 * kR * 4;
-    s.total = s.bars + 192 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
+    s.total = s.bars + 208 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
     return s;
 }
 
@@ -550,9 +550,10 @@ constexpr uint32_t kColO = 2 * kT;
 // S of tile k (the k-th of this CTA) into its buffer's columns.
 template <int NB>
 __device__ __forceinline__ bool issue_s(int rope, uint32_t sq, uint32_t sk, uint32_t b_kfull, uint32_t b_sfull,
-                                        volatile int *abort, int k, uint32_t lead)
+                                        uint32_t b_sfree, volatile int *abort, int k, uint32_t lead)
 {
     const int buf = k & 1;
+    if (k >= 2 && !wait_all(b_sfree + 8 * buf, ((k >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 13, k)) return false;
     uint32_t da = desc_k(sq), db = desc_k(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel);
     const uint32_t id = idesc(64, kT, 0), d = (uint32_t)(buf * kT);
 #pragma unroll 1
@@ -597,7 +598,7 @@ template <int NB>
 __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__ Args a)
 {
     extern __shared__ unsigned char smem_raw[];
-    __shared__ long long red[13];
+    __shared__ long long red[kThreads / 32];
     __shared__ int s_cur[8];
     const uint32_t raw = saddr(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -613,10 +614,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     // of each tile buffer and 128 latents: widened (kfull), and O^T added (pv, the last of a tile
     // standing for the tile)
     const uint32_t b_kfull = b_qfull + 16, b_pv = b_kfull + 64, b_sfull = b_pv + 64, b_pfull = b_sfull + 16;
-    const uint32_t b_drain = b_pfull + 8;
-    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 176);
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 180);
-    int *kplain = reinterpret_cast<int *>(gb + L.bars + 192);           // [2][8]
+    const uint32_t b_drain = b_pfull + 8, b_sfree = b_drain + 8;
+    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 192);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 196);
+    int *kplain = reinterpret_cast<int *>(gb + L.bars + 208);           // [2][8]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -629,7 +630,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         mbar_init(b_sfull, 1);
         mbar_init(b_sfull + 8, 1);
         mbar_init(b_pfull, 4);
-        mbar_init(b_drain, 1);
+        mbar_init(b_drain, 2);
+        mbar_init(b_sfree, 4);
+        mbar_init(b_sfree + 8, 4);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     tc_after();
     const uint32_t tmem = *tslot;
     long long lead = incl - mine, total = 0;
-    for (int i = 0; i < 13; i++) {
+    for (int i = 0; i < kThreads / 32; i++) {
         if (i < warp) lead += red[i];
         total += red[i];
     }
@@ -782,35 +785,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 write_out<NB>(a, s, (size_t)c * 2 + (slot1 ? 1 : 0), t_o, (s.rows + 15) & ~15, any, rowf, warp, lane);
             tc_before();
         }
-    } else if (warp == 12) {
-        // ------------------------------------------------------------------ MMA issuer
+    } else if (warp >= 12) {
+        // ----------------------------------------------- MMA issue: S (warp 12), O^T (warp 13)
         const uint32_t lead = elect();
         for (;;) {
             const bool have = next_seg(a, cur, s);
             if (!__any_sync(0xffffffffu, have)) break;
-            if (!wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
-            tc_after();
-            item++;
             const int nt = __reduce_max_sync(0xffffffffu, max(0, s.t1 - s.t0));
-            const uint32_t id_o = idesc(128, __reduce_max_sync(0xffffffffu, (s.rows + 15) & ~15), 1);
-            if (nt == 0) commit(b_qempty, lead);
             bool stop = false;
-            for (int i = 0; i < nt && !stop; i++) {
-                // S of tile i and, behind every second one and the last, O of the pair
-                const int k = g + i;
-                stop = !issue_s<NB>(a.d.rope, sq, sk, b_kfull, b_sfull, abort, k, lead);
-                if (stop) break;
-                if (i + 1 == nt) commit(b_qempty, lead);
-                else if (!(i & 1)) continue;
-                for (int j = i & ~1; j <= i; j++) {
-                    if (!wait_all(b_pfull, (g + j) & 1, abort, K3_SITE_CACHE4, 5, g + j)) { stop = true; break; }
-                    tc_after();
-                    issue_o<NB>(a.d.rope, sk, sp, b_pv, id_o, g + j, j ? 1u : 0u, lead);
+            if (warp == 12) {
+                if (!wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 3, item)) break;
+                tc_after();
+                item++;
+                for (int i = 0; i < nt; i++) {
+                    stop = !issue_s<NB>(a.d.rope, sq, sk, b_kfull, b_sfull, b_sfree, abort, g + i, lead);
+                    if (stop) break;
                 }
+                if (stop) break;
+                commit(b_qempty, lead);
+            } else {
+                const uint32_t id_o = idesc(128, __reduce_max_sync(0xffffffffu, (s.rows + 15) & ~15), 1);
+                for (int i = 0; i < nt; i++) {
+                    stop = !wait_all(b_pfull, (g + i) & 1, abort, K3_SITE_CACHE4, 5, g + i);
+                    if (stop) break;
+                    tc_after();
+                    issue_o<NB>(a.d.rope, sk, sp, b_pv, id_o, g + i, i ? 1u : 0u, lead);
+                }
+                if (stop) break;
             }
-            if (stop) break;
             g += nt;
         }
+        __syncwarp();
+        // every MMA of this warp has completed once this barrier flips
+        if (elect()) commit(b_drain, 1u);
         __syncwarp();
     } else {
         // --------------------------------------------------- softmax, rescale, results
@@ -841,6 +848,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 tc_after();
                 float v[32];
                 ld_s(lanes + (uint32_t)(buf * kT), v);
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_sfree + 8 * buf);
                 const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
                 const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
                 const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
@@ -975,9 +985,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         }
     }
     __syncthreads();
-    if (warp == 12 && lane == 0) {
-        // every MMA issued above has completed once this barrier flips
-        commit(b_drain, 1u);
+    if (tid == 0) {
         const long long t0 = clock64();
         while (!mbar_try(b_drain, 0)) {
             if (clock64() - t0 > kSpinLimit) { k3_raise_at(K3D_ETIMEOUT, K3_SITE_CACHE4, 12, 0, (int)blockIdx.x); break; }
