@@ -17,9 +17,8 @@
 namespace k3 {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kMaxReq = 8192;            // requests per call: 32 KB of row starts in shared memory
-constexpr int kPer = kMaxReq / kPlanThreads;
+constexpr int kMaxReq = 8192;            // requests per call: three arrays of 32 KB in shared memory
+constexpr int kMaxPer = 8;               // requests per thread at most (1024 threads)
 
 struct Plan {
     K3dPages p;
@@ -28,31 +27,32 @@ struct Plan {
     int B, N;
 };
 
-// exclusive prefix and total of one value per thread over the block
-__device__ __forceinline__ long long block_scan(long long v, long long *total, long long *part)
+// exclusive prefixes and totals of three values per thread over the block, one barrier
+struct Three { long long a, b, c; };
+
+__device__ __forceinline__ Three block_scan(Three v, Three *total, Three *part)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long s = v;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    Three s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
+        const long long x = __shfl_up_sync(0xffffffffu, s.a, o), y = __shfl_up_sync(0xffffffffu, s.b, o),
+                        z = __shfl_up_sync(0xffffffffu, s.c, o);
+        if (lane >= o) { s.a += x; s.b += y; s.c += z; }
     }
-    __syncthreads();
     if (lane == 31) part[warp] = s;
     __syncthreads();
-    long long before = 0, all = 0;
-    const int nw = blockDim.x >> 5;
+    Three before = {0, 0, 0}, all = {0, 0, 0};
     for (int i = 0; i < nw; i++) {
-        const long long t = part[i];
-        if (i < warp) before += t;
-        all += t;
+        const Three t = part[i];
+        if (i < warp) { before.a += t.a; before.b += t.b; before.c += t.c; }
+        all.a += t.a; all.b += t.b; all.c += t.c;
     }
     *total = all;
-    return before + s - v;
+    return Three{before.a + s.a - v.a, before.b + s.b - v.b, before.c + s.c - v.c};
 }
 
-// The request of row t: the last b with row_start[b] <= t (empty requests are passed over).
+// The request of row (or moved page) t: the last b with start[b] <= t (empty requests are passed over).
 __device__ __forceinline__ int request_of(const int *start, int B, int t)
 {
     int lo = 0, hi = B;                  // start[lo] <= t < start[hi]
@@ -76,89 +76,106 @@ __device__ __forceinline__ void fill_row(const Plan &a, const int *start, int t,
     a.slots[t] = slot;
 }
 
-// One CTA: the scan over the requests, the stack, the tables, and, up to a.N rows given by
-// `fill`, the rows too.
-__global__ void __launch_bounds__(kPlanThreads) k_page_plan(Plan a, int fill)
+// One CTA: the scan over the requests, the stack, the tables, and, with `fill`, the rows too.
+// The pages that move are dealt out over the threads whichever request they belong to (a
+// thread for each request took 37 us with 100 prompts of up to 128 pages). What a call needs
+// is three round trips to memory, so a small batch gets a small block.
+__global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
 {
     pdl_wait();
     pdl_trigger();
-    extern __shared__ int start[];                  // [B + 1] row starts
-    __shared__ long long part[32];
+    extern __shared__ int start[];                  // [3][B + 1]: row starts, first page taken, first given back
+    __shared__ Three part[32];
     __shared__ int s_bad;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, nt = blockDim.x;
+    int *s_grow = start + a.B + 1, *s_drop = s_grow + a.B + 1;
     if (tid == 0) s_bad = 0;
-    __syncthreads();
+    const int nf = *a.p.n_free;
     // a contiguous run of requests per thread
-    const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
+    const int per = (a.B + nt - 1) / nt;
     const int b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
-    int need[kPer], held[kPer];
-    long long grow = 0, drop = 0, rows = 0;
+    int ln[kMaxPer], nw[kMaxPer], held[kMaxPer];
+#pragma unroll
+    for (int k = 0; k < kMaxPer; k++) {
+        const bool on = b0 + k < b1;
+        ln[k] = on ? a.len[b0 + k] : 0;
+        nw[k] = on ? a.nnew[b0 + k] : 0;
+        held[k] = on ? a.p.held[b0 + k] : 0;
+    }
+    __syncthreads();                                // s_bad is set
+    Three mine = {0, 0, 0};                         // pages taken, pages given back, rows
     int bad = 0;
-    for (int k = 0; k < per && b0 + k < b1; k++) {
-        const int ln = a.len[b0 + k], nw = a.nnew[b0 + k], h = a.p.held[b0 + k];
-        const long long total = (long long)ln + nw;
-        if (ln < 0 || nw < 0 || h < 0 || h > a.p.max_pages || total > INT_MAX) {
-            bad = max(bad, K3D_PLAN_BAD);
-            need[k] = held[k] = 0;
+    auto need_of = [&](int k) { return (int)(((long long)ln[k] + nw[k] + a.p.page - 1) / a.p.page); };
+#pragma unroll
+    for (int k = 0; k < kMaxPer; k++) {
+        if (b0 + k >= b1) continue;
+        if (ln[k] < 0 || nw[k] < 0 || held[k] < 0 || held[k] > a.p.max_pages || (long long)ln[k] + nw[k] > INT_MAX) {
+            bad = K3D_PLAN_BAD;
             continue;
         }
-        const int nd = (int)((total + a.p.page - 1) / a.p.page);
-        if (nd > a.p.max_pages) bad = max(bad, K3D_PLAN_TABLE);
-        need[k] = nd;
-        held[k] = h;
-        if (nd > h) grow += nd - h; else drop += h - nd;
-        rows += nw;
+        const int need = need_of(k);
+        if (need > a.p.max_pages) bad = max(bad, K3D_PLAN_TABLE);
+        mine.a += max(0, need - held[k]);
+        mine.b += max(0, held[k] - need);
+        mine.c += nw[k];
     }
     if (bad) atomicMax(&s_bad, bad);
-    long long all_grow, all_drop, all_rows;
-    const long long g0 = block_scan(grow, &all_grow, part);
-    const long long d0 = block_scan(drop, &all_drop, part);
-    const long long r0 = block_scan(rows, &all_rows, part);
-    const int nf = *a.p.n_free;
-    __syncthreads();                                // s_bad is complete
+    Three all;
+    Three at = block_scan(mine, &all, part);        // its barrier also completes s_bad
     int code = s_bad;
     if (code == K3D_PLAN_OK) {
-        if (nf < 0 || nf + all_drop > a.p.n_pages) code = K3D_PLAN_BAD;
-        else if (all_rows > a.N) code = K3D_PLAN_ROWS;
-        else if (all_grow > nf + all_drop) code = K3D_PLAN_PAGES;
+        if (nf < 0 || nf + all.b > a.p.n_pages) code = K3D_PLAN_BAD;
+        else if (all.c > a.N) code = K3D_PLAN_ROWS;
+        else if (all.a > nf + all.b) code = K3D_PLAN_PAGES;
     }
     const bool ok = code == K3D_PLAN_OK;
     if (tid == 0) {
         *a.status = code;
-        a.row_start[a.B] = start[a.B] = ok ? (int)all_rows : 0;
+        a.row_start[a.B] = start[a.B] = ok ? (int)all.c : 0;
+        s_grow[a.B] = ok ? (int)all.a : 0;
+        s_drop[a.B] = ok ? (int)all.b : 0;
+        if (ok) *a.p.n_free = (int)(nf + all.b - all.a);
     }
     // row starts and lengths; on a failure no request has rows
-    {
-        long long r = r0;
-        for (int k = 0; k < per && b0 + k < b1; k++) {
-            const int b = b0 + k;
-            a.row_start[b] = start[b] = ok ? (int)r : 0;
-            a.kv_len[b] = ok ? a.len[b] + a.nnew[b] : 0;
-            if (ok) r += a.nnew[b];
+#pragma unroll
+    for (int k = 0; k < kMaxPer; k++) {
+        const int b = b0 + k;
+        if (b >= b1) continue;
+        a.row_start[b] = start[b] = ok ? (int)at.c : 0;
+        a.kv_len[b] = ok ? ln[k] + nw[k] : 0;
+        s_grow[b] = ok ? (int)at.a : 0;
+        s_drop[b] = ok ? (int)at.b : 0;
+        if (ok) {
+            const int need = need_of(k);
+            a.p.held[b] = need;
+            at.a += max(0, need - held[k]);
+            at.b += max(0, held[k] - need);
+            at.c += nw[k];
         }
     }
+    __syncthreads();
     if (ok) {
-        // given back: rank i of the releases in (request, page) order lies at nf + all_drop - 1 - i
-        long long d = d0;
-        for (int k = 0; k < per && b0 + k < b1; k++)
-            for (int j = need[k]; j < held[k]; j++, d++) {
-                int *e = a.p.table + (size_t)(b0 + k) * a.p.max_pages + j;
-                a.p.free_list[nf + all_drop - 1 - d] = *e;
-                *e = -1;
-            }
-        __syncthreads();
-        const long long have = nf + all_drop;
-        long long g = g0;
-        for (int k = 0; k < per && b0 + k < b1; k++) {
-            for (int j = held[k]; j < need[k]; j++, g++)
-                a.p.table[(size_t)(b0 + k) * a.p.max_pages + j] = a.p.free_list[have - 1 - g];
-            a.p.held[b0 + k] = need[k];
+        // pages after the call: the first of request b's that moved is its need (given back) or
+        // its need less what was taken
+        const int taken = (int)all.a, back = (int)all.b;
+        for (int i = tid; i < back; i += nt) {
+            const int b = request_of(s_drop, a.B, i);
+            const int need = (int)(((long long)a.kv_len[b] + a.p.page - 1) / a.p.page);
+            int *e = a.p.table + (size_t)b * a.p.max_pages + need + (i - s_drop[b]);
+            a.p.free_list[nf + back - 1 - i] = *e;
+            *e = -1;
         }
-        if (tid == 0) *a.p.n_free = (int)(have - all_grow);
+        if (back > 0) __syncthreads();              // what was given back may be taken
+        for (int i = tid; i < taken; i += nt) {
+            const int b = request_of(s_grow, a.B, i);
+            const int need = (int)(((long long)a.kv_len[b] + a.p.page - 1) / a.p.page);
+            a.p.table[(size_t)b * a.p.max_pages + need - (s_grow[b + 1] - i)] = a.p.free_list[nf + back - 1 - i];
+        }
     }
-    __syncthreads();                                // tables and row starts of the whole block
-    if (fill)
-        for (int t = tid; t < a.N; t += kPlanThreads) fill_row(a, start, t, start[a.B]);
+    if (fill) {
+        if (ok && all.a > 0) __syncthreads();       // the tables of the whole block
+        for (int t = tid; t < a.N; t += nt) fill_row(a, start, t, start[a.B]);
+    }
 }
 
 __global__ void __launch_bounds__(256) k_page_rows(Plan a)
@@ -190,9 +207,15 @@ extern "C" int k3d_page_plan(const K3dPages *p, const int *len, const int *n_new
     K3_TRY(ensure_ctx());
     const Plan a{*p, len, n_new, row_start, kv_len, pos, slots, status, B, N};
     const size_t smem = (size_t)(B + 1) * sizeof(int);
+    static unsigned long long init = 0;                // one bit per device
+    if (!(init & dev_bit())) {
+        allow_smem_max(k_page_plan);
+        init |= dev_bit();
+    }
     // Up to 4096 rows the one CTA writes them itself; above, a second launch spreads them.
     const int fill = N <= 4096 ? 1 : 0;
-    launch_pdl(k_page_plan, dim3(1), dim3(kPlanThreads), smem, stream(), a, fill);
+    const int threads = B <= 256 && N <= 1024 ? 256 : 1024;
+    launch_pdl(k_page_plan, dim3(1), dim3(threads), 3 * smem, stream(), a, fill);
     note_launch();
     K3_TRY(check_launch("page plan"));
     if (!fill) {
