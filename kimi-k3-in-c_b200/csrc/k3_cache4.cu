@@ -89,11 +89,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const 
     const int lane = threadIdx.x & 31;
     const int r = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
     if (r >= N) return;
-    const int slot = slots[r];
-    if (slot < 0 || slot >= d.n_pages * d.page) {
-        if (slot != -1 && lane == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, r, slot, 0);
-        return;
-    }
+    const int slot = slots[r];                       // on its way together with the row
     const T *src = x + (size_t)r * ldx;
     const bool own = lane * 16 < d.kv, ropes = 2 * lane < d.rope;
     float v[16], rv[2] = {0.f, 0.f};
@@ -103,6 +99,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const 
     if (ropes) {
         rv[0] = to_f(src[d.kv + 2 * lane]);
         rv[1] = to_f(src[d.kv + 2 * lane + 1]);
+    }
+    if (slot < 0 || slot >= d.n_pages * d.page) {
+        if (slot != -1 && lane == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, r, slot, 0);
+        return;
     }
     float amax = 0.f, rmax = fmaxf(fabsf(rv[0]), fabsf(rv[1]));
     bool fine = fabsf(rv[0]) <= 3.4028234e38f && fabsf(rv[1]) <= 3.4028234e38f;

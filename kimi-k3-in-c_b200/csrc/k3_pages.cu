@@ -17,7 +17,7 @@
 namespace k3 {
 namespace {
 
-constexpr int kMaxReq = 8192;            // requests per call: three arrays of 32 KB in shared memory
+constexpr int kMaxReq = 8192;            // requests per call: four arrays of 32 KB in shared memory
 constexpr int kMaxPer = 8;               // requests per thread at most (1024 threads)
 
 struct Plan {
@@ -84,11 +84,11 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
 {
     pdl_wait();
     pdl_trigger();
-    extern __shared__ int start[];                  // [3][B + 1]: row starts, first page taken, first given back
+    extern __shared__ int start[];                  // [4][B + 1]: row starts, first page taken, first given back, need
     __shared__ Three part[32];
     __shared__ int s_bad;
     const int tid = threadIdx.x, nt = blockDim.x;
-    int *s_grow = start + a.B + 1, *s_drop = s_grow + a.B + 1;
+    int *s_grow = start + a.B + 1, *s_drop = s_grow + a.B + 1, *s_need = s_drop + a.B + 1;
     if (tid == 0) s_bad = 0;
     const int nf = *a.p.n_free;
     // a contiguous run of requests per thread
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
         s_drop[b] = ok ? (int)at.b : 0;
         if (ok) {
             const int need = need_of(k);
-            a.p.held[b] = need;
+            a.p.held[b] = s_need[b] = need;
             at.a += max(0, need - held[k]);
             at.b += max(0, held[k] - need);
             at.c += nw[k];
@@ -158,18 +158,19 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
         // pages after the call: the first of request b's that moved is its need (given back) or
         // its need less what was taken
         const int taken = (int)all.a, back = (int)all.b;
+#pragma unroll 4
         for (int i = tid; i < back; i += nt) {
             const int b = request_of(s_drop, a.B, i);
-            const int need = (int)(((long long)a.kv_len[b] + a.p.page - 1) / a.p.page);
-            int *e = a.p.table + (size_t)b * a.p.max_pages + need + (i - s_drop[b]);
+            int *e = a.p.table + (size_t)b * a.p.max_pages + s_need[b] + (i - s_drop[b]);
             a.p.free_list[nf + back - 1 - i] = *e;
             *e = -1;
         }
         if (back > 0) __syncthreads();              // what was given back may be taken
+#pragma unroll 4
         for (int i = tid; i < taken; i += nt) {
+            const int page = a.p.free_list[nf + back - 1 - i];
             const int b = request_of(s_grow, a.B, i);
-            const int need = (int)(((long long)a.kv_len[b] + a.p.page - 1) / a.p.page);
-            a.p.table[(size_t)b * a.p.max_pages + need - (s_grow[b + 1] - i)] = a.p.free_list[nf + back - 1 - i];
+            a.p.table[(size_t)b * a.p.max_pages + s_need[b] - (s_grow[b + 1] - i)] = page;
         }
     }
     if (fill) {
@@ -178,15 +179,47 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
     }
 }
 
-__global__ void __launch_bounds__(256) k_page_rows(Plan a)
+// Four consecutive rows to a thread: they share a search for their request most of the time,
+// and go out as 16 bytes where the arrays allow it.
+__global__ void __launch_bounds__(256) k_page_rows(Plan a, int vec)
 {
     pdl_wait();
     pdl_trigger();
     extern __shared__ int start[];
     for (int i = threadIdx.x; i <= a.B; i += blockDim.x) start[i] = a.row_start[i];
     __syncthreads();
-    for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < a.N; t += gridDim.x * blockDim.x)
-        fill_row(a, start, t, start[a.B]);
+    const int rows = start[a.B];
+    for (int t0 = (blockIdx.x * blockDim.x + threadIdx.x) * 4; t0 < a.N; t0 += gridDim.x * blockDim.x * 4) {
+        int pos[4], slot[4], b = -1, end = 0, ln = 0, pg = -1, page = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int t = t0 + k;
+            pos[k] = slot[k] = -1;
+            if (t >= rows) continue;
+            if (b < 0 || t >= end) {
+                b = request_of(start, a.B, t);
+                end = start[b + 1];
+                ln = a.len[b] - start[b];
+                pg = -1;
+            }
+            pos[k] = ln + t;
+            const int q = pos[k] / a.p.page;
+            if (q != pg) {
+                pg = q;
+                page = a.p.table[(size_t)b * a.p.max_pages + q];
+            }
+            slot[k] = page * a.p.page + (pos[k] - q * a.p.page);
+        }
+        if (vec && t0 + 4 <= a.N) {
+            *reinterpret_cast<int4 *>(a.pos + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<int4 *>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        } else {
+            for (int k = 0; k < 4 && t0 + k < a.N; k++) {
+                a.pos[t0 + k] = pos[k];
+                a.slots[t0 + k] = slot[k];
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -215,13 +248,14 @@ extern "C" int k3d_page_plan(const K3dPages *p, const int *len, const int *n_new
     // Up to 4096 rows the one CTA writes them itself; above, a second launch spreads them.
     const int fill = N <= 4096 ? 1 : 0;
     const int threads = B <= 256 && N <= 1024 ? 256 : 1024;
-    launch_pdl(k_page_plan, dim3(1), dim3(threads), 3 * smem, stream(), a, fill);
+    launch_pdl(k_page_plan, dim3(1), dim3(threads), 4 * smem, stream(), a, fill);
     note_launch();
     K3_TRY(check_launch("page plan"));
     if (!fill) {
         const int most = 8 * sm_count();
-        const int grid = (N + 255) / 256;
-        launch_pdl(k_page_rows, dim3(grid < most ? grid : most), dim3(256), smem, stream(), a);
+        const int grid = (N + 1023) / 1024;
+        const int vec = !(((uintptr_t)pos | (uintptr_t)slots) & 15u) ? 1 : 0;
+        launch_pdl(k_page_rows, dim3(grid < most ? grid : most), dim3(256), smem, stream(), a, vec);
         note_launch();
         K3_TRY(check_launch("page rows"));
     }

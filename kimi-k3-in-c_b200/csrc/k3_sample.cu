@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kVMax, 2) k_spec_verify(Verify a)
         total = xt;
         before = lane < rank ? xt : 0;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
+        for (int o = 8; o > 0; o >>= 1) {
             total += __shfl_xor_sync(0xffffffffu, total, o);
             before += __shfl_xor_sync(0xffffffffu, before, o);
         }
@@ -435,6 +435,35 @@ __global__ void __launch_bounds__(kVMax, 2) k_spec_verify(Verify a)
     }
 }
 
+// CTAs to a row: sixteen (more than the portable eight) while the rows take no more than half
+// of the SMs so, eight while they leave SMs idle, else `many`; fewer where a CTA would have
+// less than 2048 elements.
+int cluster_of(int rows, int V, int many)
+{
+    int cs = (long long)rows * 32 <= sm_count() ? 16 : (long long)rows * 8 <= 4 * sm_count() ? 8 : many;
+    while (cs > 1 && V < cs * 2048) cs >>= 1;
+    return cs;
+}
+
+// Lets a kernel run in clusters of sixteen; set once per kernel and device.
+int wide_clusters(const void *f)
+{
+    static const void *done[64][8];
+    int d = 0;
+    cudaGetDevice(&d);
+    for (const void *&e : done[d & 63]) {
+        if (e == f) return K3D_OK;
+        if (e) continue;
+        if (cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+            cudaGetLastError();
+            return fail(K3D_ECUDA, "clusters of sixteen CTAs");
+        }
+        e = f;
+        return K3D_OK;
+    }
+    return K3D_OK;
+}
+
 }  // namespace
 }  // namespace k3
 
@@ -451,11 +480,11 @@ int k3d_logits_softmax(float *p, const float *logits, const float *temp, int row
         return fail(K3D_EINVAL, "k3d_logits_softmax: unaligned pointer");
     if ((long long)rows * 8 > 0x7fffffffLL) return fail(K3D_EINVAL, "k3d_logits_softmax: %d rows", rows);
     K3_TRY(ensure_ctx());
-    // eight CTAs to a row while the rows leave SMs idle, else four (320 rows of 163840: 88 us with four,
-    // 97 with two, 106 with eight);
-    // fewer where a CTA would have less than 2048 elements
-    int cs = (long long)rows * 8 <= 4 * sm_count() ? 8 : 4;
-    while (cs > 1 && vocab < cs * 2048) cs >>= 1;
+    // four CTAs to a row where the rows fill the card (320 rows of 163840: 88 us with four, 97
+    // with two, 106 with eight)
+    const int cs = cluster_of(rows, vocab, 4);
+    K3_TRY(wide_clusters(vec4(p) && vec4(logits) && vocab % 4 == 0 ? (const void *)k_logits_softmax<true>
+                                                                    : (const void *)k_logits_softmax<false>));
     const int chunk = ((vocab + cs - 1) / cs + 3) & ~3;
     const bool vec = vec4(p) && vec4(logits) && vocab % 4 == 0;
     launch_pdl_cluster(vec ? k_logits_softmax<true> : k_logits_softmax<false>, dim3(rows * cs), dim3(kSmThreads), 0, stream(),
@@ -477,8 +506,9 @@ int k3d_spec_verify(int *tokens, int *n_accept, const float *target, const float
         return fail(K3D_EINVAL, "k3d_spec_verify: unaligned pointer");
     if ((long long)B * 8 > 0x7fffffffLL) return fail(K3D_EINVAL, "k3d_spec_verify: B %d", B);
     K3_TRY(ensure_ctx());
-    int cs = 8;
-    while (cs > 1 && vocab < cs * 2048) cs >>= 1;
+    const int cs = cluster_of(B, vocab, 8);
+    K3_TRY(wide_clusters(vec4(target) && vec4(draft) && vocab % 4 == 0 ? (const void *)k_spec_verify<true>
+                                                                        : (const void *)k_spec_verify<false>));
     Verify a{tokens, n_accept, target, K > 0 ? draft : nullptr, ids, n_draft, u_accept, u_sample, B, K, vocab,
              ((vocab + cs - 1) / cs + 3) & ~3, cs};
     const bool vec = vec4(target) && vec4(draft) && vocab % 4 == 0;
