@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
     __syncthreads();                                // s_bad is set
     Three mine = {0, 0, 0};                         // pages taken, pages given back, rows
     int bad = 0;
-    auto need_of = [&](int k) { return (int)(((long long)ln[k] + nw[k] + a.p.page - 1) / a.p.page); };
+    // of lengths that add up to 31 bits; 32-bit unsigned, so the rounding up does not overflow
+    auto need_of = [&](int k) { return (int)(((uint32_t)ln[k] + (uint32_t)nw[k] + (uint32_t)a.p.page - 1u) / (uint32_t)a.p.page); };
 #pragma unroll
     for (int k = 0; k < kMaxPer; k++) {
         if (b0 + k >= b1) continue;
@@ -158,19 +159,41 @@ __global__ void __launch_bounds__(1024) k_page_plan(Plan a, int fill)
         // pages after the call: the first of request b's that moved is its need (given back) or
         // its need less what was taken
         const int taken = (int)all.a, back = (int)all.b;
-#pragma unroll 4
-        for (int i = tid; i < back; i += nt) {
-            const int b = request_of(s_drop, a.B, i);
-            int *e = a.p.table + (size_t)b * a.p.max_pages + s_need[b] + (i - s_drop[b]);
-            a.p.free_list[nf + back - 1 - i] = *e;
-            *e = -1;
+        // eight at a time: all the reads, then the writes (the compiler cannot tell that they do
+        // not meet, and would wait for each read)
+        for (int i0 = tid; i0 < back; i0 += 8 * nt) {
+            int *e[8], page[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = i0 + k * nt;
+                e[k] = nullptr;
+                if (i < back) {
+                    const int b = request_of(s_drop, a.B, i);
+                    e[k] = a.p.table + (size_t)b * a.p.max_pages + s_need[b] + (i - s_drop[b]);
+                    page[k] = *e[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (e[k]) {
+                    a.p.free_list[nf + back - 1 - (i0 + k * nt)] = page[k];
+                    *e[k] = -1;
+                }
         }
         if (back > 0) __syncthreads();              // what was given back may be taken
-#pragma unroll 4
-        for (int i = tid; i < taken; i += nt) {
-            const int page = a.p.free_list[nf + back - 1 - i];
-            const int b = request_of(s_grow, a.B, i);
-            a.p.table[(size_t)b * a.p.max_pages + s_need[b] - (s_grow[b + 1] - i)] = page;
+        for (int i0 = tid; i0 < taken; i0 += 8 * nt) {
+            int page[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (i0 + k * nt < taken) page[k] = a.p.free_list[nf + back - 1 - (i0 + k * nt)];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = i0 + k * nt;
+                if (i < taken) {
+                    const int b = request_of(s_grow, a.B, i);
+                    a.p.table[(size_t)b * a.p.max_pages + s_need[b] - (s_grow[b + 1] - i)] = page[k];
+                }
+            }
         }
     }
     if (fill) {
@@ -190,25 +213,27 @@ __global__ void __launch_bounds__(256) k_page_rows(Plan a, int vec)
     __syncthreads();
     const int rows = start[a.B];
     for (int t0 = (blockIdx.x * blockDim.x + threadIdx.x) * 4; t0 < a.N; t0 += gridDim.x * blockDim.x * 4) {
-        int pos[4], slot[4], b = -1, end = 0, ln = 0, pg = -1, page = 0;
+        int pos[4], slot[4], b = -1, end = 0, p = 0, q = 0, in = 0, base = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int t = t0 + k;
             pos[k] = slot[k] = -1;
             if (t >= rows) continue;
+            bool turn = false;                      // another page
             if (b < 0 || t >= end) {
                 b = request_of(start, a.B, t);
                 end = start[b + 1];
-                ln = a.len[b] - start[b];
-                pg = -1;
+                p = a.len[b] + t - start[b];
+                q = (int)((uint32_t)p / (uint32_t)a.p.page);
+                in = p - q * a.p.page;
+                turn = true;
+            } else {
+                p++;
+                if (++in == a.p.page) { in = 0; q++; turn = true; }
             }
-            pos[k] = ln + t;
-            const int q = pos[k] / a.p.page;
-            if (q != pg) {
-                pg = q;
-                page = a.p.table[(size_t)b * a.p.max_pages + q];
-            }
-            slot[k] = page * a.p.page + (pos[k] - q * a.p.page);
+            if (turn) base = a.p.table[(size_t)b * a.p.max_pages + q] * a.p.page;
+            pos[k] = p;
+            slot[k] = base + in;
         }
         if (vec && t0 + 4 <= a.N) {
             *reinterpret_cast<int4 *>(a.pos + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
