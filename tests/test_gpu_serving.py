@@ -541,3 +541,160 @@ def test_verify_draws_the_distribution(k3):
                     g.random((B, 1)).astype(np.float32), g.random(B).astype(np.float32))
     count = np.bincount(got[:, 0], minlength=V)
     assert (np.abs(count - B * p) <= 5 * np.sqrt(B * p * (1 - p))).all(), count
+
+
+# ------------------------------------------------------------------------ a serving step ----
+class Loop:
+    """One step of a serving loop as one run of calls on fixed buffers: plan the pages, store the
+    new rows, attend, probabilities of the rows' logits, verify the drafts."""
+
+    def __init__(self, lib, g, B=5, K=3, H=16, kv=256, rope=32, page=16, n_pages=90, V=700):
+        self.lib, self.g, self.B, self.K, self.H, self.kv, self.w, self.page, self.V = lib, g, B, K, H, kv, kv + rope, page, V
+        self.N = B * (K + 1)
+        self.shape = k3cuda.K3dCache4(kv, rope, page, n_pages)
+        self.pool = DevBuf(lib.k3d_cache4_bytes(self.shape))
+        check(lib.k3d_memset(self.pool.ptr, 0xff, self.pool.nbytes))
+        self.free = g.permutation(n_pages).tolist()
+        self.pages = DevPages(lib, page, n_pages, 12, B, self.free)
+        self.host = ref.Pages(page, n_pages, 12, B, self.free)
+        f = np.float32
+        self.dev = {k: DevBuf.from_array(np.zeros(s, t)) for k, s, t in (
+            ("len", B, np.int32), ("new", B, np.int32), ("start", B + 1, np.int32), ("kvl", B, np.int32),
+            ("pos", self.N, np.int32), ("slots", self.N, np.int32), ("status", 1, np.int32),
+            ("x", (self.N, self.w), f), ("q", (self.N, H, self.w), f), ("o", (self.N, H, kv), f),
+            ("logits", (self.N, V), f), ("p", (self.N, V), f), ("temp", self.N, f), ("draft", (B, K, V), f),
+            ("ids", (B, K), np.int32), ("nd", B, np.int32), ("u", (B, K), f), ("us", B, f),
+            ("tok", (B, K + 1), np.int32), ("acc", B, np.int32))}
+        self.nws = lib.k3d_mla_attend4_ws_bytes(self.shape, B, self.N, H)
+        self.ws = DevBuf(self.nws)
+
+    def inputs(self, lens, new):
+        g, B, K, V = self.g, self.B, self.K, self.V
+        h = {"len": np.int32(lens), "new": np.int32(new), "x": rows(g, self.N, self.w, 0.5),
+             "q": from_bf16(to_bf16(g.standard_normal((self.N, self.H, self.w)))), "nd": np.int32([n - 1 for n in new]),
+             "logits": (g.standard_normal((self.N, V)) * 3).astype(np.float32),
+             "temp": np.where(g.random(self.N) < 0.3, 0, 0.8).astype(np.float32), "draft": chances(g, (B, K, V)),
+             "ids": g.integers(0, V, (B, K)).astype(np.int32), "u": (g.random((B, K)) * 0.3).astype(np.float32),
+             "us": g.random(B).astype(np.float32)}
+        for k, v in h.items():
+            self.dev[k].upload(v)
+        return h
+
+    def calls(self):
+        lib, d = self.lib, {k: b.ptr for k, b in self.dev.items()}
+        check(lib.k3d_page_plan(self.pages.p, d["len"], d["new"], self.B, self.N, d["start"], d["kvl"], d["pos"],
+                                d["slots"], d["status"]))
+        check(lib.k3d_cache4_store(self.shape, self.pool.ptr, d["x"], F32, self.w, d["slots"], self.N))
+        check(lib.k3d_mla_attend4(d["o"], F32, d["q"], F32, self.shape, self.pool.ptr, self.pages.t.ptr, 12, d["start"],
+                                  d["kvl"], self.B, self.N, self.H, 0.07, self.ws.ptr, self.nws))
+        check(lib.k3d_logits_softmax(d["p"], d["logits"], d["temp"], self.N, self.V))
+        # a request's target rows lie K + 1 apart: here every request brings K + 1 rows
+        check(lib.k3d_spec_verify(d["tok"], d["acc"], d["p"], d["draft"], d["ids"], d["nd"], d["u"], d["us"], self.B,
+                                  self.K, self.V))
+
+    def results(self):
+        shapes = {"start": (np.int32, self.B + 1), "kvl": (np.int32, self.B), "slots": (np.int32, self.N),
+                  "o": (np.float32, (self.N, self.H, self.kv)), "p": (np.float32, (self.N, self.V)),
+                  "tok": (np.int32, (self.B, self.K + 1)), "acc": (np.int32, self.B), "status": (np.int32, 1)}
+        return {k: self.dev[k].download(*v) for k, v in shapes.items()}
+
+
+def run_steps(k3, graph):
+    g = np.random.default_rng(21)
+    L = Loop(k3, g)
+    B, K = L.B, L.K
+    lens = np.zeros(B, int)
+    known = [np.zeros((0, L.w)) for _ in range(B)]            # what the oracle's cache holds
+    out, ex = [], None
+    for step in range(6):
+        new = [K + 1] * B
+        h = L.inputs(lens, new)
+        if graph and ex is None:
+            check(k3.k3d_graph_begin())
+            L.calls()
+            ex = k3.k3d_graph_end()
+            assert ex
+        if graph:
+            check(k3.k3d_graph_launch(ex))
+        else:
+            L.calls()
+        check(k3.k3d_sync())
+        r = L.results()
+        code, start, kvl, _, slots = L.host.plan(lens.tolist(), new, L.N)
+        assert code == 0 and r["status"][0] == 0
+        assert r["start"].tolist() == start and r["kvl"].tolist() == kvl and r["slots"].tolist() == slots
+        same_pages(L.pages, L.host)
+        values = ref.quantise(h["x"], L.kv)[1]
+        for b in range(B):
+            known[b] = np.concatenate([known[b][:lens[b]], values[start[b]:start[b + 1]]])
+            want = ref.attend(h["q"][start[b]:start[b + 1]], known[b], L.kv, 0.07, new[b])
+            # fp32 results: the weights' and the scores' rounding as in Batch.compare, for values
+            # of up to about 10 and scores' sums of magnitudes of up to 0.07 x 300 x 4
+            assert np.abs(r["o"][start[b]:start[b + 1]] - want).max() <= 10 * (2.0 ** -11 + np.expm1(2 * 84 * (2.0 ** -11 + 288 * 2.0 ** -24)))
+        softmax_close(r["p"], h["logits"], h["temp"])
+        tok, acc = ref.verify(r["p"].reshape(B, K + 1, L.V), h["draft"], h["ids"], h["nd"], h["u"], h["us"])
+        assert np.array_equal(r["tok"], tok) and np.array_equal(r["acc"], acc)
+        lens = lens + acc + 1                                  # the rejected drafts' rows are given up
+        if step == 3:
+            lens[1] = 0                                        # a request that ended, another in its place
+            known[1] = known[1][:0]
+        out.append({k: v.copy() for k, v in r.items()})
+    if ex:
+        k3.k3d_graph_destroy(ex)
+    return out
+
+
+def test_serving_steps_and_their_graph(k3):
+    """Six steps against the definitions, called one by one and as a graph that is replayed with
+    new contents of the same buffers: the same bits."""
+    eager, graph = run_steps(k3, False), run_steps(k3, True)
+    for a, b in zip(eager, graph):
+        for k in a:
+            assert np.array_equal(a[k], b[k]), k
+
+
+def test_serving_step_on_another_stream(k3):
+    """The calls run on the stream that k3d_set_stream names."""
+    rt = ctypes.CDLL("libcudart.so.12")
+    s = ctypes.c_void_p()
+    assert rt.cudaStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+    own = k3.k3d_stream()
+    try:
+        check(k3.k3d_sync())
+        check(k3.k3d_set_stream(s))
+        got = run_steps(k3, False)
+    finally:
+        check(k3.k3d_sync())
+        check(k3.k3d_set_stream(own))
+        rt.cudaStreamDestroy(s)
+    want = run_steps(k3, False)
+    for a, b in zip(got, want):
+        for k in a:
+            assert np.array_equal(a[k], b[k]), k
+
+
+def test_attend_bits_do_not_depend_on_the_run(k3):
+    """Splits, merges and launches in one order: the same bits every time."""
+    B = Batch(k3, 512, 64, 64, [(5000, 2), (700, 1), (64, 3)], seed=31)
+    q = B.queries(64, 6, 1.0, BF16)
+    first = B.call(q, 64, 6, BF16, F32, 0.07)
+    for _ in range(5):
+        assert np.array_equal(first, B.call(q, 64, 6, BF16, F32, 0.07))
+
+
+def test_attend_lengths_that_do_not_fit(k3):
+    """A kv_len above max_pages * page, or row_starts that run past N, raise the device error; the
+    rows of the other requests are right."""
+    B = Batch(k3, 256, 32, 16, [(40, 1), (30, 1)], seed=32)
+    B.bufs[2] = i32([10 ** 6, 30])
+    q = B.queries(16, 2, 1.0, BF16)
+    got = B.call(q, 16, 2, BF16, F32, 0.07, sync=False)
+    assert k3.k3d_sync() == k3cuda.K3D_EDEVICE
+    k3.k3d_clear_status()
+    want = ref.attend(q[1:2], B.values[1], 256, 0.07, 1)
+    assert np.abs(got[1:2] - want).max() <= 2.0 ** -6
+    B.bufs[1], B.bufs[2] = i32([0, 1, 9]), i32([40, 30])
+    got = B.call(q, 16, 2, BF16, F32, 0.07, sync=False)
+    assert k3.k3d_sync() == k3cuda.K3D_EDEVICE
+    k3.k3d_clear_status()
+    assert np.abs(got[:1] - ref.attend(q[:1], B.values[0], 256, 0.07, 1)).max() <= 2.0 ** -6
