@@ -8,9 +8,13 @@
 // positions (none: zeros).
 //
 // WORK. The rows of a request are contiguous in q ([N][H] flattened); an item is up to 64 of
-// them (whole tokens when H <= 64, else 64 heads of one token) and a unit is one item times
-// one tile of 64 positions. The units of all items, item-major, are cut into one contiguous
-// range per CTA, so ragged lengths balance themselves. An item that one CTA covers is written
+// them (whole tokens when H <= 64, else 64 heads of one token). An item counts one unit for
+// each tile of 64 positions and four for its start (Q, the first tile's way through the
+// pipeline and the result take about as long as four tiles: 10 us against 2.4), the units of
+// all items, item-major, are cut into one contiguous range per CTA, and a cut that falls into
+// an item's start moves to its beginning. So ragged lengths balance themselves: 128 us -> 99
+// us for 16 ragged requests of four tokens against ranges of tiles alone, where a CTA that
+// met four items took 126 us and the average one 84. An item that one CTA covers is written
 // directly; the parts of a cut item (at most two per CTA) go to the workspace as
 // (unnormalised o, max, sum) and a second kernel adds them in CTA order.
 //
@@ -55,6 +59,7 @@ constexpr int kR = 64;                    // rows per item
 constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
 constexpr int kThreads = 448;
 constexpr int kMaxUnits = 1 << 30;
+constexpr int kStart = 4;                 // units that an item counts beside its tiles
 constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
 constexpr float kStep = 8.f;              // m moves when a tile passes it by this
 constexpr int kUnit = -2;                 // the fp16 operand is in units of 2^kUnit
@@ -136,17 +141,17 @@ struct Cursor {
 __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
 {
     if (c.u >= c.u1) return false;
-    while (c.u >= c.pre + c.r.items * c.r.tiles) {
-        c.pre += c.r.items * c.r.tiles;
+    while (c.u >= c.pre + c.r.items * (c.r.tiles + kStart)) {
+        c.pre += c.r.items * (c.r.tiles + kStart);
         c.b++;
         c.r = request(a, c.b);
     }
-    const int item = (int)((uint32_t)(c.u - c.pre) / (uint32_t)c.r.tiles);
+    const int item = (int)((uint32_t)(c.u - c.pre) / (uint32_t)(c.r.tiles + kStart));
     s.b = c.b;
     s.n = c.r.n;
     s.kvl = c.r.kvl;
-    s.begin = c.pre + item * c.r.tiles;
-    s.end = s.begin + c.r.tiles;
+    s.begin = c.pre + item * (c.r.tiles + kStart);
+    s.end = s.begin + c.r.tiles + kStart;
     const int first = c.r.first;
     int last;
     if (a.hc == 1) {
@@ -163,8 +168,8 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
     }
     const int stop = min(c.u1, s.end);
     const int seen = max(0, c.r.kvl - c.r.n + last + 1);
-    s.t0 = c.u - s.begin;
-    s.t1 = min(stop - s.begin, (seen + kT - 1) / kT);
+    s.t0 = max(0, c.u - s.begin - kStart);
+    s.t1 = min(stop - s.begin - kStart, (seen + kT - 1) / kT);
     s.whole = c.u == s.begin && stop == s.end;
     c.u = stop;
     return true;
@@ -599,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
 {
     extern __shared__ unsigned char smem_raw[];
     __shared__ long long red[kThreads / 32];
-    __shared__ int s_cur[8];
+    __shared__ int s_cur[10];
     const uint32_t raw = saddr(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     unsigned char *gb = smem_raw + (base - raw);
@@ -650,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     long long mine = 0;
     for (int b = rb0; b < rb1; b++) {
         const Req r = request(a, b);
-        mine += (long long)r.items * r.tiles;
+        mine += (long long)r.items * (r.tiles + kStart);
     }
     long long incl = mine;
 #pragma unroll
@@ -676,20 +681,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     const int c = blockIdx.x;
     // the first U % G CTAs take one unit more than the others
     const int each = G > 0 ? (int)((uint32_t)U / (uint32_t)G) : 0, more = U - each * G;
-    const int u0 = c < G ? c * each + min(c, more) : 0, u1 = c < G ? u0 + each + (c < more ? 1 : 0) : 0;
-    if (u0 < u1 && u0 >= before && u0 < before + mine) {
-        int pre = before;
-        for (int b = rb0; b < rb1; b++) {
-            const Req r = request(a, b);
-            if (u0 < pre + r.items * r.tiles) { 
-                s_cur[0] = b; s_cur[1] = pre; s_cur[2] = r.first; s_cur[3] = r.n;
-                s_cur[4] = r.kvl; s_cur[5] = r.items; s_cur[6] = r.tiles;
-                break;
+    const int cut0 = c < G ? c * each + min(c, more) : 0, cut1 = c < G ? cut0 + each + (c < more ? 1 : 0) : 0;
+    if (tid == 0) s_cur[7] = cut0, s_cur[8] = cut1;
+    __syncthreads();
+    // the thread whose requests hold a cut: the request, and the cut moved out of an item's start
+    for (int k = 0; k < 2; k++) {
+        const int cut = k ? cut1 : cut0;
+        if (cut0 < cut1 && cut >= before && cut < before + mine) {
+            int pre = before;
+            for (int b = rb0; b < rb1; b++) {
+                const Req r = request(a, b);
+                const int len = r.tiles + kStart;
+                if (cut < pre + r.items * len) {
+                    const int begin = pre + (int)((uint32_t)(cut - pre) / (uint32_t)len) * len;
+                    s_cur[7 + k] = cut - begin <= kStart ? begin : cut;
+                    if (k == 0) {
+                        s_cur[0] = b; s_cur[1] = pre; s_cur[2] = r.first; s_cur[3] = r.n;
+                        s_cur[4] = r.kvl; s_cur[5] = r.items; s_cur[6] = r.tiles;
+                    }
+                    break;
+                }
+                pre += r.items * len;
             }
-            pre += r.items * r.tiles;
         }
     }
     __syncthreads();
+    const int u0 = s_cur[7], u1 = s_cur[8];
     Cursor cur;
     cur.u = u0;
     cur.u1 = u1;
@@ -701,14 +718,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         cur.r.items = s_cur[5]; cur.r.tiles = s_cur[6];
     }
     if (tid == 12 * 32) {
-        int4 i0 = make_int4(u0, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
+        // an empty range (its cuts moved together) keeps its place in the order
+        int4 i0 = make_int4(c < G ? u0 : 0x7fffffff, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
         Cursor t = cur;
         Seg s;
         if (next_seg(a, t, s)) {
-            i0 = make_int4(u0, s.begin, s.end, 0);
+            i0.y = s.begin;
+            i0.z = s.end;
             i1 = make_int4(s.row0, s.rows, 0, 0);
-        } else {
-            i0.x = 0x7fffffff;
         }
         a.info[2 * c] = i0;
         a.info[2 * c + 1] = i1;
