@@ -41,7 +41,7 @@
 //
 // ROLES (416 threads): warps 0-7 load a tile ahead into registers, widen and store it;
 // warps 8-11 do the softmax and the rescaling; these 12 load Q and write the results; warp
-// 12 issues the MMAs in the order S(t + 1), O(t). A tile is handed over in pieces of 128
+// 12 issues the MMAs in the order S(t + 1), O(t). A tile is handed over in pieces of 256
 // latents: O(t) frees a piece of the buffer, the widening of tile t + 2 fills it while O(t)
 // goes on, and S(t + 2) follows it, so that the softmax of tile t + 1 has the length of O(t)
 // and S(t + 2) to run in. Every wait is bounded (k3_bulk.cuh).
@@ -80,6 +80,10 @@ struct Args {
     float2 *ml;                           // [grid][2][64] (max, sum), base 2
     int4 *info;                           // [grid][2]: {u0, item begin, item end, 0}, {row0, rows, 0, 0}
 };
+
+// Pieces of 256 latents in which a tile is handed over.
+template <int NB>
+__host__ __device__ constexpr int pieces() { return (NB + 1) / 2; }
 
 struct Smem {                             // offsets from the 1024-byte aligned base
     uint32_t q, k, p, kinfo, row, bars, total;
@@ -293,6 +297,14 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b)
 {
     uint32_t r;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// two values rounded to bf16, x in the low half
+__device__ __forceinline__ uint32_t bf16x2(float x, float y)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
     return r;
 }
 
@@ -534,8 +546,7 @@ __device__ __forceinline__ void write_out(const Args &a, const Seg &s, size_t sl
                     if (a.out_f32) {
                         *reinterpret_cast<float2 *>((float *)a.out + at) = make_float2(x, y);
                     } else {
-                        *reinterpret_cast<uint32_t *>((uint16_t *)a.out + at) =
-                            (uint32_t)f32_to_bf16_bits(x) | ((uint32_t)f32_to_bf16_bits(y) << 16);
+                        *reinterpret_cast<uint32_t *>((uint16_t *)a.out + at) = bf16x2(x, y);
                     }
                 }
             }
@@ -563,7 +574,7 @@ __device__ __forceinline__ bool issue_s(int rope, uint32_t sq, uint32_t sk, uint
     const uint32_t id = idesc(64, kT, 0), d = (uint32_t)(buf * kT);
 #pragma unroll 1
     for (int i = 0; i < NB; i++) {
-        if (!wait_all(b_kfull + 8 * (buf * 4 + i), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+        if (!(i & 1) && !wait_all(b_kfull + 8 * (buf * 2 + (i >> 1)), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
         tc_after();
 #pragma unroll
         for (int p = 0; p < 2; p++) {
@@ -580,22 +591,24 @@ __device__ __forceinline__ bool issue_s(int rope, uint32_t sq, uint32_t sk, uint
     return true;
 }
 
-// O^T += V^T P^T of tile k; every 128 latents that have been used are given back.
+// O^T += V^T P^T of tile k; every 256 latents that have been used are given back.
 template <int NB>
 __device__ __forceinline__ void issue_o(int rope, uint32_t sk, uint32_t sp, uint32_t b_pv, uint32_t id, int k, uint32_t accum,
                                         uint32_t lead)
 {
     const int buf = k & 1;
-    uint32_t da = desc_mn(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel, kPanel), d = kColO, bar = b_pv + 32 * buf;
+    uint32_t da = desc_mn(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel, kPanel), d = kColO, bar = b_pv + 16 * buf;
     const uint32_t db = desc_k(sp);
 #pragma unroll 1
     for (int blk = 0; blk < NB; blk++) {
 #pragma unroll
         for (int k4 = 0; k4 < kT / 16; k4++) mma(d, da + 128 * k4, db + 2 * k4, id, k4 ? 1u : accum, lead);
-        commit(bar, lead);
+        if ((blk & 1) || blk == NB - 1) {
+            commit(bar, lead);
+            bar += 8;
+        }
         da += 2 * kPanel / 16;
         d += kR;
-        bar += 8;
     }
 }
 
@@ -616,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     float *rowf = reinterpret_cast<float *>(gb + L.row + 2 * kR * 4);   // rescale factors, then 1 / sum
     int *flags = reinterpret_cast<int *>(gb + L.row + 3 * kR * 4);      // [2][4]
     const uint32_t b_qfull = base + L.bars, b_qempty = b_qfull + 8;
-    // of each tile buffer and 128 latents: widened (kfull), and O^T added (pv, the last of a tile
+    // of each tile buffer and 256 latents: widened (kfull), and O^T added (pv, the last of a tile
     // standing for the tile)
     const uint32_t b_kfull = b_qfull + 16, b_pv = b_kfull + 64, b_sfull = b_pv + 64, b_pfull = b_sfull + 16;
     const uint32_t b_drain = b_pfull + 8, b_sfree = b_drain + 8;
@@ -777,12 +790,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 const float res = r.e < 0 ? __int_as_float(0xff800000)
                                 : r.e == 255 ? __int_as_float(0x7fc00000) : (float)(e - min(max(e, kUnit - kDown), kUnit));
                 const int plain = __all_sync(0xffffffffu, res == 0.f);
-                // as soon as O(g - 2) has used 128 latents of the buffer, this tile's take their place
+                // as soon as O(g - 2) has used 256 latents of the buffer, this tile's take their place
 #pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 4 + i), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
-                    widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
-                    if (i == NB - 1) {
+                for (int h = 0; h < pieces<NB>(); h++) {
+                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 2 + h), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
+#pragma unroll
+                    for (int i = 2 * h; i < 2 * h + 2 && i < NB; i++)
+                        widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
+                    if (h == pieces<NB>() - 1) {
                         const uint32_t pan = tile + 2 * NB * kPanel;
                         if (part < a.d.rope / 8)
                             sts16(pan + rope0, make_uint4(hmul2(r.rope[0].x, up), hmul2(r.rope[0].y, up), hmul2(r.rope[0].z, up), hmul2(r.rope[0].w, up)));
@@ -793,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     }
                     async_fence();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(b_kfull + 8 * (buf * 4 + i));
+                    if (lane == 0) mbar_arrive(b_kfull + 8 * (buf * 2 + h));
                 }
             }
             named_sync(2, 384);                           // the item's sums are written, O^T is complete
@@ -859,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
                 const int buf = g & 1;
-                if (!dead && !(wait_all(b_kfull + 8 * (buf * 4 + NB - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                if (!dead && !(wait_all(b_kfull + 8 * (buf * 2 + pieces<NB>() - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
                                wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
                     dead = true;
                 tc_after();
@@ -947,7 +962,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
                 if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
                 // O(t - 1) has been added: P may be written, and the accumulator rescaled
-                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
                 tc_after();
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
@@ -992,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     a.ml[slot * kR + rb] = make_float2(mb, sumb);
                 }
             }
-            if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 4 + NB - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
             tc_after();
             tc_before();
             named_sync(2, 384);
