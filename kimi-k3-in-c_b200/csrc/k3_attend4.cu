@@ -59,7 +59,7 @@ constexpr int kR = 64;                    // rows per item
 constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
 constexpr int kThreads = 448;
 constexpr int kMaxUnits = 1 << 30;
-constexpr int kStart = 4;                 // units that an item counts beside its tiles
+constexpr int kStart = 5;                 // units that an item counts beside its tiles
 constexpr float kLift = 7.f;              // P = 2^(a - m + 7)
 constexpr float kStep = 8.f;              // m moves when a tile passes it by this
 constexpr int kUnit = -2;                 // the fp16 operand is in units of 2^kUnit
