@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
     const float T = temp ? temp[r] : 1.0f;
     const float NEG = __int_as_float(0xff800000), POS = __int_as_float(0x7f800000);
     const bool greedy = !(T > 0.f);
-    const float c = 1.4426950408889634f / T;
+    const float c = fminf(1.4426950408889634f / T, 3.4028234e38f);   // finite at a subnormal T: 0 c stays 0
     constexpr int W = VEC ? 4 : 1, U = VEC ? 10 : 20, nw = kSmThreads / 32;   // values of a load, loads of a step
     // e^((t - m) / T); minus infinity is 0 at any temperature, an infinite one too
     auto weigh = [&](float t, float m) { return t > NEG ? ex2((t - m) * c) : 0.f; };

@@ -455,6 +455,17 @@ def test_softmax_masked_rows(k3):
     assert (hot[0, ::2] == 0).all() and np.allclose(hot[0, 1::2], 1 / 4500, rtol=1e-6)
 
 
+def test_softmax_at_the_ends_of_the_temperatures(k3):
+    """1 / T leaves fp32 below 2^-128: the maxima share the whole, as they do at any T so small."""
+    g = np.random.default_rng(5)
+    x = g.standard_normal((5, 5000)).astype(np.float32)
+    x[:, [3, 4001]] = 6.0
+    temp = np.array([1e-45, 1e-40, 1e-30, 1e30, 3e38], np.float32)
+    got = softmax(k3, x, temp)
+    softmax_close(got, x, temp)
+    assert (got[:3, 3] == 0.5).all() and (got[:3, 4001] == 0.5).all()
+
+
 # ------------------------------------------------------------------------ verification ----
 def verify(lib, target, draft, ids, nd, u, us):
     B, K1, V = target.shape
