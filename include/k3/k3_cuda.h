@@ -532,7 +532,7 @@ int    k3d_logits_softmax(float *p, const float *logits, const float *temp, int 
  * so that the result does not depend on the order of the sum. Where max(p - q, 0) is nothing
  * anywhere the draw is from p. tokens [B][K + 1] receives the kept drafts, the drawn token (-1
  * where p holds nothing either) and -1 behind it. A draft id outside the vocabulary is never
- * kept. */
+ * kept. vocab is below 2^19, so that the sums of any row stay within 63 bits. */
 int    k3d_spec_verify(int *tokens, int *n_accept, const float *target, const float *draft,
                        const int *ids, const int *n_draft, const float *u_accept,
                        const float *u_sample, int B, int K, int vocab);

@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
 constexpr int kVMax = 512;                // threads
 constexpr int kVParts = 4;
 constexpr int kMaxDraft = 32;
+constexpr int kMaxVocab = 1 << 19;        // as many weights of 2^44 add up to 2^63: no row of p overflows the sums
 
 struct Verify {
     int *tokens, *n_accept;
@@ -496,8 +497,8 @@ int k3d_logits_softmax(float *p, const float *logits, const float *temp, int row
 int k3d_spec_verify(int *tokens, int *n_accept, const float *target, const float *draft, const int *ids,
                     const int *n_draft, const float *u_accept, const float *u_sample, int B, int K, int vocab)
 {
-    if (B < 0 || K < 0 || K > kMaxDraft || vocab < 1)
-        return fail(K3D_EINVAL, "k3d_spec_verify: B %d, K %d (0 to %d), vocab %d", B, K, kMaxDraft, vocab);
+    if (B < 0 || K < 0 || K > kMaxDraft || vocab < 1 || vocab >= kMaxVocab)
+        return fail(K3D_EINVAL, "k3d_spec_verify: B %d, K %d (0 to %d), vocab %d (below %d)", B, K, kMaxDraft, vocab, kMaxVocab);
     if (B == 0) return K3D_OK;
     if (!tokens || !n_accept || !target || !u_sample || (K > 0 && (!ids || !u_accept)))
         return fail(K3D_EINVAL, "k3d_spec_verify null pointer");

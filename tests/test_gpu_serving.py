@@ -539,6 +539,16 @@ def test_verify_edges(k3):
     assert want[1][0] == 2 and want[1][7] == 0 and want[0][2, 0] == -1
 
 
+def test_verify_largest_sums(k3):
+    """A row of ones over the largest vocabulary: the running sum ends just below 2^63."""
+    V = (1 << 19) - 1
+    target = np.ones((2, 1, V), np.float32)
+    ids, u, us = np.zeros((2, 0)), np.zeros((2, 0)), np.array([0.5, 1.0 - 2.0 ** -24])
+    want = ref.verify(target, None, ids, None, u, us)
+    got = verify(k3, target, None, np.zeros((2, 1)), None, np.zeros((2, 1)), us)
+    assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+
+
 def test_verify_draws_the_distribution(k3):
     """Drafts from q, verified against p, come out distributed as p: 4096 requests over six
     tokens. The count of a token is binomial, so five standard deviations bound it but for one

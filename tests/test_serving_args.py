@@ -113,6 +113,11 @@ def test_softmax_and_verify(lib):
     assert call(B=0, tok=None) == OK
 
 
+def test_verify_vocabularies_whose_sums_overflow(lib):
+    for v in (1 << 19, (1 << 31) - 1):
+        assert lib.k3d_spec_verify(A, A, A, A, A, A, A, A, 2, 4, v) == EINVAL
+
+
 def test_without_a_gpu_valid_calls_fail_loudly(lib):
     import glob
     if glob.glob("/dev/nvidia[0-9]*"):
