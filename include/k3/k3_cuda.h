@@ -440,7 +440,8 @@ int    k3d_a2a_plan(const int *idx, int TK, int n_experts, int nranks, int *cnt,
  * the latent cache held in 4 bits, attention over it, and tokens drawn from the logits. No
  * reference counterpart except where noted: the CPU engine holds one sequence in one
  * contiguous fp32 cache and takes the argmax. As everywhere here: device pointers,
- * asynchronous on the library stream, no allocation, capturable into a CUDA graph. */
+ * asynchronous on the library stream, no allocation, capturable into a CUDA graph. Counts of
+ * rows, pages and vocabulary entries are at most 2^30. */
 
 /* Page tables and slot maps of B requests (at most 8192) in one plan. Request b holds `len`
  * positions and brings n_new[b] more (0 is allowed); after the call it holds exactly
@@ -510,8 +511,10 @@ int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtyp
  * softmax and sums are fp32; q is rounded to fp16 in units of its row (exact for bf16) and
  * the softmax weights to fp16. A page id outside the pool, a kv_len above max_pages * page,
  * or a row_start that is not a prefix sum within N raises K3D_EBOUND; such positions count as
- * not there. The workspace belongs to the call until it has run: two calls that may run at
- * the same time (two streams, two graphs) need one each. */
+ * not there. A call whose tiles of 64 positions, counted for every 64 rows, pass 2^30 raises
+ * it too and writes nothing. Weights below about 2^-31 of a row's largest count as 0. N H and
+ * max_pages * page are at most 2^30. The workspace belongs to the call until it has run: two
+ * calls that may run at the same time (two streams, two graphs) need one each. */
 size_t k3d_mla_attend4_ws_bytes(const K3dCache4 *c, int B, int N, int H);
 int    k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const K3dCache4 *c,
                        const void *pool, const int *table, int max_pages, const int *row_start,

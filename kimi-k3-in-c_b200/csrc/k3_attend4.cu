@@ -1233,8 +1233,10 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
                     float scale, void *ws, size_t ws_bytes)
 {
     K3_TRY(cache4_check(c, "k3d_mla_attend4"));
-    if (B < 1 || N < 0 || H < 1 || H > 1024 || max_pages < 1 || (long long)max_pages * c->page > 0x7fffffffLL ||
-        (long long)N * H > 0x7fffffffLL)
+    // positions, rows and requests are counted in 31 bits, with a tile to spare
+    constexpr long long kMost = 1LL << 30;
+    if (B < 1 || B > kMost || N < 0 || H < 1 || H > 1024 || max_pages < 1 || (long long)max_pages * c->page > kMost ||
+        (long long)N * H > kMost)
         return fail(K3D_EINVAL, "k3d_mla_attend4: B %d, N %d, H %d (1 to 1024), max_pages %d", B, N, H, max_pages);
     for (int t : {out_dtype, q_dtype})
         if (t != K3D_DT_F32 && t != K3D_DT_BF16)

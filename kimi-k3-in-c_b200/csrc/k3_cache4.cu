@@ -233,7 +233,7 @@ int rows_check(const K3dCache4 *c, const void *pool, const void *x, int dtype, s
                const char *who)
 {
     K3_TRY(cache4_check(c, who));
-    if (N < 0) return fail(K3D_EINVAL, "%s: %d rows", who, N);
+    if (N < 0 || N > 1 << 30) return fail(K3D_EINVAL, "%s: %d rows (up to 2^30)", who, N);
     if (dtype != K3D_DT_F32 && dtype != K3D_DT_BF16)
         return fail(K3D_EUNSUPPORTED, "%s: rows are K3D_DT_F32 or K3D_DT_BF16, not %d", who, dtype);
     if (ld < (size_t)(c->kv_lora + c->qk_rope))

@@ -257,11 +257,15 @@ extern "C" int k3d_page_plan(const K3dPages *p, const int *len, const int *n_new
 {
     if (!p || !p->table || !p->held || !p->free_list || !p->n_free || !len || !n_new || !row_start || !kv_len || !status)
         return fail(K3D_EINVAL, "k3d_page_plan null pointer");
-    if (p->page < 1 || p->n_pages < 1 || p->max_pages < 1 || (long long)p->page * p->n_pages > INT_MAX)
+    if (p->page < 1 || p->n_pages < 1 || p->n_pages > 1 << 30 || p->max_pages < 1 || (long long)p->page * p->n_pages > INT_MAX)
         return fail(K3D_EINVAL, "k3d_page_plan: page %d, n_pages %d, max_pages %d (slots are 31-bit)", p->page,
                     p->n_pages, p->max_pages);
     if (B < 1 || B > kMaxReq) return fail(K3D_EINVAL, "k3d_page_plan: %d requests (1 to %d)", B, kMaxReq);
-    if (N < 0 || (N > 0 && (!pos || !slots))) return fail(K3D_EINVAL, "k3d_page_plan: %d rows", N);
+    if (N < 0 || N > 1 << 30 || (N > 0 && (!pos || !slots))) return fail(K3D_EINVAL, "k3d_page_plan: %d rows", N);
+    if (((uintptr_t)p->table | (uintptr_t)p->held | (uintptr_t)p->free_list | (uintptr_t)p->n_free | (uintptr_t)len |
+         (uintptr_t)n_new | (uintptr_t)row_start | (uintptr_t)kv_len | (uintptr_t)pos | (uintptr_t)slots |
+         (uintptr_t)status) & 3u)
+        return fail(K3D_EINVAL, "k3d_page_plan: unaligned pointer");
     K3_TRY(ensure_ctx());
     const Plan a{*p, len, n_new, row_start, kv_len, pos, slots, status, B, N};
     const size_t smem = (size_t)(B + 1) * sizeof(int);

@@ -474,7 +474,7 @@ extern "C" {
 
 int k3d_logits_softmax(float *p, const float *logits, const float *temp, int rows, int vocab)
 {
-    if (rows < 0 || vocab < 1) return fail(K3D_EINVAL, "k3d_logits_softmax: %d rows of %d", rows, vocab);
+    if (rows < 0 || vocab < 1 || vocab > 1 << 30) return fail(K3D_EINVAL, "k3d_logits_softmax: %d rows of %d", rows, vocab);
     if (rows == 0) return K3D_OK;
     if (!p || !logits) return fail(K3D_EINVAL, "k3d_logits_softmax null pointer");
     if (((uintptr_t)p | (uintptr_t)logits | (uintptr_t)temp) & 3u)

@@ -118,6 +118,34 @@ def test_verify_vocabularies_whose_sums_overflow(lib):
         assert lib.k3d_spec_verify(A, A, A, A, A, A, A, A, 2, 4, v) == EINVAL
 
 
+def test_counts_beyond_31_bits(lib):
+    s, big = shape(), (1 << 30) + 1
+    n = lib.k3d_mla_attend4_ws_bytes(s, 2, 3, 64)
+
+    def attend(max_pages=4, B=2, N=3, H=64):
+        return lib.k3d_mla_attend4(A, BF16, A, BF16, s, A, A, max_pages, A, A, B, N, H, 0.1, A, n)
+
+    for kw in (dict(max_pages=(1 << 24) + 1), dict(B=big), dict(N=big, H=1), dict(N=(1 << 24) + 1)):
+        assert attend(**kw) == EINVAL, kw
+    assert lib.k3d_cache4_store(s, A, A, F32, 576, A, big) == EINVAL
+    assert lib.k3d_cache4_load(s, A, A, F32, 576, A, big) == EINVAL
+    assert lib.k3d_logits_softmax(A, A, None, 1, big) == EINVAL
+    p = k3cuda.K3dPages(64, 100, 10, A, A, A, A)
+    assert lib.k3d_page_plan(p, A, A, 4, big, A, A, A, A, A) == EINVAL
+    p = k3cuda.K3dPages(1, big, 10, A, A, A, A)
+    assert lib.k3d_page_plan(p, A, A, 4, 8, A, A, A, A, A) == EINVAL
+
+
+def test_plan_arrays_are_whole_ints(lib):
+    for i in range(7):
+        args = [A + 2 if i == k else A for k in range(7)]
+        p = k3cuda.K3dPages(64, 100, 10, A, A, A, A)
+        assert lib.k3d_page_plan(p, args[0], args[1], 4, 8, *args[2:]) == EINVAL
+    for i in range(4):
+        p = k3cuda.K3dPages(64, 100, 10, *(A + 1 if i == k else A for k in range(4)))
+        assert lib.k3d_page_plan(p, A, A, 4, 8, A, A, A, A, A) == EINVAL
+
+
 def test_without_a_gpu_valid_calls_fail_loudly(lib):
     import glob
     if glob.glob("/dev/nvidia[0-9]*"):
