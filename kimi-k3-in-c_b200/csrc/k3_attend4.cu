@@ -9,14 +9,15 @@
 //
 // WORK. The rows of a request are contiguous in q ([N][H] flattened); an item is up to 64 of
 // them (whole tokens when H <= 64, else 64 heads of one token). An item counts one unit for
-// each tile of 64 positions and four for its start (Q, the first tile's way through the
-// pipeline and the result take about as long as four tiles: 10 us against 2.4), the units of
-// all items, item-major, are cut into one contiguous range per CTA, and a cut that falls into
-// an item's start moves to its beginning. So ragged lengths balance themselves: 128 us -> 99
-// us for 16 ragged requests of four tokens against ranges of tiles alone, where a CTA that
-// met four items took 126 us and the average one 84. An item that one CTA covers is written
-// directly; the parts of a cut item (at most two per CTA) go to the workspace as
-// (unnormalised o, max, sum) and a second kernel adds them in CTA order.
+// each tile of 64 positions and five for its start (Q, the first tile's way through the
+// pipeline and the result take about as long as five tiles, 10 us), the units of all items,
+// item-major, are cut into one contiguous range per CTA, and a cut that falls into an item's
+// start moves to its beginning. So ragged lengths balance themselves: 142 -> 114 us for 16
+// ragged requests of four tokens, 64 heads, up to 8192 positions, against ranges of tiles
+// alone, where a CTA that met four items took half as long again as the average one. An item
+// that one CTA covers is written directly; the parts of a cut item (at most two per CTA) go to
+// the workspace as (unnormalised o, max, sum) and a second kernel adds them in CTA order.
+// Units are numbered in 31 bits: a call of more than 2^30 raises K3D_EBOUND.
 //
 // PRODUCTS (tcgen05, fp16 x fp16, fp32 accumulators in tensor memory). A tile's rows are
 // widened once to fp16, 64 values to a 128-byte swizzled panel row, and serve both products
@@ -39,12 +40,24 @@
 // moves only when a tile's maximum passes it by 2^8, so the accumulator is rescaled rarely;
 // P stays below 2^15 and weights down to 2^-21 of the largest keep all their bits.
 //
-// ROLES (416 threads): warps 0-7 load a tile ahead into registers, widen and store it;
+// ROLES (448 threads): warps 0-7 load a tile ahead into registers, widen and store it;
 // warps 8-11 do the softmax and the rescaling; these 12 load Q and write the results; warp
-// 12 issues the MMAs in the order S(t + 1), O(t). A tile is handed over in pieces of 256
-// latents: O(t) frees a piece of the buffer, the widening of tile t + 2 fills it while O(t)
-// goes on, and S(t + 2) follows it, so that the softmax of tile t + 1 has the length of O(t)
-// and S(t + 2) to run in. Every wait is bounded (k3_bulk.cuh).
+// 12 issues S, warp 13 O^T. A tile is handed over in pieces of 256 latents: O(t) frees a piece
+// of the buffer, the widening of tile t + 2 fills it while O(t) goes on, and S(t + 2) follows
+// it, so that the softmax of tile t + 1 has the length of O(t) and S(t + 2) to run in. Every
+// wait is bounded (k3_bulk.cuh).
+//
+// BOUND. A tile of 64 positions x 576 values takes about 3200 cycles, of which the widening's
+// instructions are the largest part and the shared memory (74 KB written, then read once by
+// S and once by O^T) at least 2600; the tensor pipe is busy a third of the time. 512 + 64, one
+// library call:
+//   64 requests, one token, 16 heads, up to 8192 positions    72 us
+//   16 requests, four tokens, 64 heads, up to 8192 positions 103 us
+//   one request, one token, 64 heads: 1000 positions 21 us, 32768 positions 33 us
+// One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
+// Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
+// that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
+// again), and Q by all 14 warps in one batch (121 us where 103 are).
 #include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"

@@ -76,9 +76,9 @@ __device__ __forceinline__ int unit_exp(float a, float m, int le)
 }
 
 // One warp per row, lane l the 16-value block l of the latent and rope elements 2l, 2l + 1.
-// All loads are issued before the row's maximum is formed; the codes are 7 exact
-// comparisons |y| against t s (t a midpoint of two codes, s four significant bits), so no
-// quotient is rounded onto a tie. Traffic bound for prompts (2304 or 1152 bytes in, 417
+// All loads are issued before the row's maximum is formed; the code's three
+// bits are exact comparisons of |y| with t s (t a midpoint of two codes, s four significant
+// bits), so no quotient is rounded onto a tie. Traffic bound for prompts (2304 or 1152 bytes in, 417
 // out per row at 512 + 64), one memory round trip for a decode step.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const T *x, size_t ldx,
@@ -124,16 +124,17 @@ __global__ void __launch_bounds__(32 * kRowWarps) k_cache4_store(Pool4 d, const 
     if (own) {
         const float ay = fine ? amax * up * up2 : 0.f;
         const __nv_fp8_storage_t sb = __nv_cvt_float_to_fp8(__fdiv_rn(ay, 6.0f), __NV_SATFINITE, __NV_E4M3);
-        const float s = e4m3_to_f32(sb);
+        // a scale of 0: nothing is above its midpoints
+        const float s0 = e4m3_to_f32(sb), s = s0 > 0.f ? s0 : __int_as_float(0x7f800000);
         uint32_t w[2] = {0u, 0u};
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const float y = fine ? v[i] * up * up2 : 0.f;
             const float a = fabsf(y);
-            uint32_t c = (a > 0.25f * s) + (a >= 0.75f * s) + (a > 1.25f * s) + (a >= 1.75f * s) +
-                         (a > 2.5f * s) + (a >= 3.5f * s) + (a > 5.0f * s);
-            if (!(s > 0.f)) c = 0u;
-            c |= (__float_as_uint(y) >> 28) & 8u;
+            const bool b2 = a >= 1.75f * s;
+            const bool b1 = a >= (b2 ? 3.5f * s : 0.75f * s);
+            const bool b0 = a > (b2 ? (b1 ? 5.0f * s : 2.5f * s) : (b1 ? 1.25f * s : 0.25f * s));
+            const uint32_t c = ((__float_as_uint(y) >> 28) & 8u) | (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (b0 ? 1u : 0u);
             w[i >> 3] |= c << (4 * (i & 7));
         }
         *reinterpret_cast<uint2 *>(base + (size_t)in * (d.kv / 2) + lane * 8) = make_uint2(w[0], w[1]);
