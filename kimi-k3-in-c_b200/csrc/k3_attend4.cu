@@ -313,6 +313,14 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b)
     return r;
 }
 
+// the larger of a >= 0 and |b|, of two bf16 values each (a NaN gives way)
+__device__ __forceinline__ uint32_t absmax_bf16x2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\tabs.bf16x2 t, %2;\n\tmax.bf16x2 %0, %1, t;\n\t}" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // two values rounded to bf16, x in the low half
 __device__ __forceinline__ uint32_t bf16x2(float x, float y)
 {
@@ -481,12 +489,22 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
                 }
             };
             float m = 0.f;
+            if (F32) {
 #pragma unroll
-            for (int c = 0; c < 3; c++) {
-                float v[8];
-                value(c, v);
+                for (int c = 0; c < 3; c++) {
+                    float v[8];
+                    value(c, v);
 #pragma unroll
-                for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[k]));
+                    for (int k = 0; k < 8; k++) m = fmaxf(m, fabsf(v[k]));
+                }
+            } else {
+                uint32_t t = 0u;                          // two at a time
+#pragma unroll
+                for (int c = 0; c < 3; c++) {
+                    const uint4 x = raw[i][c][0];
+                    t = absmax_bf16x2(absmax_bf16x2(absmax_bf16x2(absmax_bf16x2(t, x.x), x.y), x.z), x.w);
+                }
+                m = fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
             }
             m = warp_max(m);
             // m < 2^e; a row with an infinity or a NaN stays as it is
