@@ -110,8 +110,8 @@ __host__ __device__ inline Smem smem_layout(int kv, int rope)
     s.k = s.q + panels * kPanel;
     s.p = s.k + 2 * panels * kPanel;
     s.kinfo = s.p + kR * 128;             // float [2][64]: residual of each position
-    s.row = s.kinfo + 2 * kT * 4;         // float [64] score factor, int [64] limit, float [64] x 2
-    s.bars = s.row + 4 * kR * 4;
+    s.row = s.kinfo + 2 * kT * 4;         // int [64] exponents of Q's rows, float [64] factors, int [2][4] flags
+    s.bars = s.row + 2 * kR * 4 + 32;
     s.total = s.bars + 208 + 64;          // barriers, then int [2][8]: a warp's rows have no residual
     return s;
 }
@@ -447,11 +447,11 @@ __device__ __forceinline__ void widen(uint2 lo, uint2 hi, uint2 scale, uint32_t 
 }
 
 // ------------------------------------------------------------------------------- Q ----
-// Rows warp, warp + 12, ... of the item: fp16 in units of 2^x (the
-// row's largest value in [2^13, 2^14)), the score factor and the number of positions the row
-// sees. Rows behind the last are zeros that see everything: they cost no case of their own.
+// Rows warp, warp + 12, ... of the item: fp16 in units of 2^(e - 14), e the row's exponent (its
+// largest value in [2^13, 2^14)), which the softmax takes into its factor. Rows behind the last
+// are zeros that see everything: they cost no case of their own.
 template <bool F32>
-__device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
+__device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_t sq, int *rexp, int warp, int lane)
 {
     constexpr int RB = F32 ? 1 : 3;                       // rows in flight (36 registers or 24)
     const int W = a.d.kv + a.d.rope, chunks = W / 8;
@@ -526,22 +526,30 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
                     sts16(sq + (uint32_t)(ch >> 3) * kPanel + swz(r, ch & 7), make_uint4(h[0], h[1], h[2], h[3]));
                 }
             }
-            if (lane == 0) {
-                // |scale| log2(e) 2^(e - 14 + kUnit), the power in two factors (it may be below -126)
-                const int k = e - 14 + kUnit, k1 = k >> 1;
-                fac[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
-                         __uint_as_float((uint32_t)(k - k1 + 127) << 23);
-                const int j = s.j0 + (a.hc == 1 ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
-                lim[r] = r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
-            }
+            if (lane == 0) rexp[r] = e;
         }
     }
 }
 
-__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, float *fac, int *lim, int warp, int lane)
+__device__ __forceinline__ void load_q(const Args &a, const Seg &s, uint32_t sq, int *rexp, int warp, int lane)
 {
-    if (a.q_f32) load_q_rows<true>(a, s, sq, fac, lim, warp, lane);
-    else load_q_rows<false>(a, s, sq, fac, lim, warp, lane);
+    if (a.q_f32) load_q_rows<true>(a, s, sq, rexp, warp, lane);
+    else load_q_rows<false>(a, s, sq, rexp, warp, lane);
+}
+
+// |scale| log2(e) 2^(e - 14 + kUnit), the power in two factors (it may be below -126)
+__device__ __forceinline__ float score_factor(const Args &a, int e)
+{
+    const int k = e - 14 + kUnit, k1 = k >> 1;
+    return fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(k1 + 127) << 23) *
+           __uint_as_float((uint32_t)(k - k1 + 127) << 23);
+}
+
+// the positions that row r of the item sees
+__device__ __forceinline__ int sees(const Args &a, const Seg &s, int r)
+{
+    const int j = s.j0 + (a.hc == 1 ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
+    return r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
 }
 
 // This warp's third of an item's result: the 16-row groups sub, sub + 3, ... of its quarter of
@@ -655,10 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     const Smem L = smem_layout(NB * 128, a.d.rope);
     const uint32_t panels = NB * 2 + (a.d.rope ? 1 : 0);
     float *kinfo = reinterpret_cast<float *>(gb + L.kinfo);
-    float *fac = reinterpret_cast<float *>(gb + L.row);
-    int *lim = reinterpret_cast<int *>(gb + L.row + kR * 4);
-    float *rowf = reinterpret_cast<float *>(gb + L.row + 2 * kR * 4);   // rescale factors, then 1 / sum
-    int *flags = reinterpret_cast<int *>(gb + L.row + 3 * kR * 4);      // [2][4]
+    int *rexp = reinterpret_cast<int *>(gb + L.row);                    // exponents of Q's rows
+    float *rowf = reinterpret_cast<float *>(gb + L.row + kR * 4);       // rescale factors, then 1 / sum
+    int *flags = reinterpret_cast<int *>(gb + L.row + 2 * kR * 4);      // [2][4]
     const uint32_t b_qfull = base + L.bars, b_qempty = b_qfull + 8;
     // of each tile buffer and 256 latents: widened (kfull), and O^T added (pv, the last of a tile
     // standing for the tile)
@@ -802,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 look_up(at, table, s.kvl);
             }
             if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 1, item)) dead = true;
-            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
+            if (!dead) load_q(a, s, sq, rexp, warp, lane);
             async_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_qfull);
@@ -892,15 +899,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         while (next_seg(a, cur, s)) {
             const bool slot1 = item > 0;
             if (item > 0 && !dead && !wait_all(b_qempty, (item - 1) & 1, abort, K3_SITE_CACHE4, 6, item)) dead = true;
-            if (!dead) load_q(a, s, sq, fac, lim, warp, lane);
+            if (!dead) load_q(a, s, sq, rexp, warp, lane);
             async_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_qfull);
             if (!dead && !wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
             item++;
             const int NR = (s.rows + 15) & ~15;
-            const float fa = fac[ra], fb = fac[rb];
-            const int la = lim[ra], lb = lim[rb];
+            const float fa = score_factor(a, rexp[ra]), fb = score_factor(a, rexp[rb]);
+            const int la = sees(a, s, ra), lb = sees(a, s, rb);
             const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
