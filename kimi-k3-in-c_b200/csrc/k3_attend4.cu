@@ -697,16 +697,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         tc_before();
     }
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = *tslot;
     pdl_wait();
     pdl_trigger();
 
-    // ---- this CTA's units: the requests' totals, then the request that holds the first unit
-    const int per = (a.B + kThreads - 1) / kThreads;
-    const int rb0 = min(a.B, tid * per), rb1 = min(a.B, rb0 + per);
+    // ---- this CTA's units: the requests' totals, then the request that holds the first unit. Up
+    // to 32 requests every warp does it for itself, a request to a lane; more are dealt out over
+    // the block, which meets three times (2 us with one request, of a call's 20).
+    Cursor cur;
+    cur.b = 0; cur.pre = 0;
+    cur.r = Req{0, 0, 0, 0, 1};
+    const int c = blockIdx.x;
+    const bool few = a.B <= 32;
+    const int per = few ? 1 : (a.B + kThreads - 1) / kThreads, me = few ? lane : tid;
+    const int rb0 = min(a.B, me * per), rb1 = min(a.B, rb0 + per);
     long long mine = 0;
+    Req r0 = cur.r;
     for (int b = rb0; b < rb1; b++) {
-        const Req r = request(a, b);
-        mine += (long long)r.items * (r.tiles + kStart);
+        r0 = request(a, b);
+        mine += (long long)r0.items * (r0.tiles + kStart);
     }
     long long incl = mine;
 #pragma unroll
@@ -714,14 +725,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         const long long t = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += t;
     }
-    if (lane == 31) red[warp] = incl;
-    __syncthreads();
-    tc_after();
-    const uint32_t tmem = *tslot;
-    long long lead = incl - mine, total = 0;
-    for (int i = 0; i < kThreads / 32; i++) {
-        if (i < warp) lead += red[i];
-        total += red[i];
+    long long lead = incl - mine, total = __shfl_sync(0xffffffffu, incl, 31);
+    if (!few) {
+        if (lane == 31) red[warp] = incl;
+        __syncthreads();
+        total = 0;
+        for (int i = 0; i < kThreads / 32; i++) {
+            if (i < warp) lead += red[i];
+            total += red[i];
+        }
     }
     if (total > kMaxUnits) {                              // unit numbers are 31-bit
         if (tid == 0) k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, a.N, a.H, 4);
@@ -729,45 +741,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     }
     const int U = (int)total, before = (int)min(lead, (long long)kMaxUnits);
     const int G = min((int)gridDim.x, U);
-    const int c = blockIdx.x;
     // the first U % G CTAs take one unit more than the others
     const int each = G > 0 ? (int)((uint32_t)U / (uint32_t)G) : 0, more = U - each * G;
     const int cut0 = c < G ? c * each + min(c, more) : 0, cut1 = c < G ? cut0 + each + (c < more ? 1 : 0) : 0;
-    if (tid == 0) s_cur[7] = cut0, s_cur[8] = cut1;
-    __syncthreads();
-    // the thread whose requests hold a cut: the request, and the cut moved out of an item's start
-    for (int k = 0; k < 2; k++) {
-        const int cut = k ? cut1 : cut0;
-        if (cut0 < cut1 && cut >= before && cut < before + mine) {
-            int pre = before;
-            for (int b = rb0; b < rb1; b++) {
-                const Req r = request(a, b);
-                const int len = r.tiles + kStart;
-                if (cut < pre + r.items * len) {
-                    const int begin = pre + (int)((uint32_t)(cut - pre) / (uint32_t)len) * len;
-                    s_cur[7 + k] = cut - begin <= kStart ? begin : cut;
-                    if (k == 0) {
-                        s_cur[0] = b; s_cur[1] = pre; s_cur[2] = r.first; s_cur[3] = r.n;
-                        s_cur[4] = r.kvl; s_cur[5] = r.items; s_cur[6] = r.tiles;
+    cur.u = cut0;
+    cur.u1 = cut1;
+    // a cut in the request of `r` whose units begin at `pre`, moved out of an item's start
+    auto moved_cut = [&](int cut, int pre, int tiles) {
+        const int len = tiles + kStart, begin = pre + (int)((uint32_t)(cut - pre) / (uint32_t)len) * len;
+        return cut - begin <= kStart ? begin : cut;
+    };
+    if (few) {
+        if (cut0 < cut1) {
+            const unsigned at0 = __ballot_sync(0xffffffffu, incl > cut0), at1 = __ballot_sync(0xffffffffu, incl > cut1);
+            const int l0 = __ffs(at0) - 1, l1 = at1 ? __ffs(at1) - 1 : 0;
+            cur.b = l0;
+            cur.pre = __shfl_sync(0xffffffffu, before, l0);
+            cur.r.first = __shfl_sync(0xffffffffu, r0.first, l0);
+            cur.r.n = __shfl_sync(0xffffffffu, r0.n, l0);
+            cur.r.kvl = __shfl_sync(0xffffffffu, r0.kvl, l0);
+            cur.r.items = __shfl_sync(0xffffffffu, r0.items, l0);
+            cur.r.tiles = __shfl_sync(0xffffffffu, r0.tiles, l0);
+            cur.u = moved_cut(cut0, cur.pre, cur.r.tiles);
+            const int pre1 = __shfl_sync(0xffffffffu, before, l1), tiles1 = __shfl_sync(0xffffffffu, r0.tiles, l1);
+            if (at1) cur.u1 = moved_cut(cut1, pre1, tiles1);
+        }
+    } else {
+        if (tid == 0) s_cur[7] = cut0, s_cur[8] = cut1;
+        __syncthreads();
+        // the thread whose requests hold a cut: the request, and where the cut moves
+        for (int k = 0; k < 2; k++) {
+            const int cut = k ? cut1 : cut0;
+            if (cut0 < cut1 && cut >= before && cut < before + mine) {
+                int pre = before;
+                for (int b = rb0; b < rb1; b++) {
+                    const Req r = request(a, b);
+                    const int len = r.tiles + kStart;
+                    if (cut < pre + r.items * len) {
+                        s_cur[7 + k] = moved_cut(cut, pre, r.tiles);
+                        if (k == 0) {
+                            s_cur[0] = b; s_cur[1] = pre; s_cur[2] = r.first; s_cur[3] = r.n;
+                            s_cur[4] = r.kvl; s_cur[5] = r.items; s_cur[6] = r.tiles;
+                        }
+                        break;
                     }
-                    break;
+                    pre += r.items * len;
                 }
-                pre += r.items * len;
             }
         }
+        __syncthreads();
+        cur.u = s_cur[7];
+        cur.u1 = s_cur[8];
+        if (cut0 < cut1) {
+            cur.b = s_cur[0];
+            cur.pre = s_cur[1];
+            cur.r.first = s_cur[2]; cur.r.n = s_cur[3]; cur.r.kvl = s_cur[4];
+            cur.r.items = s_cur[5]; cur.r.tiles = s_cur[6];
+        }
     }
-    __syncthreads();
-    const int u0 = s_cur[7], u1 = s_cur[8];
-    Cursor cur;
-    cur.u = u0;
-    cur.u1 = u1;
-    cur.b = 0; cur.pre = 0;
-    if (u0 < u1) {
-        cur.b = s_cur[0];
-        cur.pre = s_cur[1];
-        cur.r.first = s_cur[2]; cur.r.n = s_cur[3]; cur.r.kvl = s_cur[4];
-        cur.r.items = s_cur[5]; cur.r.tiles = s_cur[6];
-    }
+    const int u0 = cur.u;
     if (tid == 12 * 32) {
         // an empty range (its cuts moved together) keeps its place in the order
         int4 i0 = make_int4(c < G ? u0 : 0x7fffffff, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
