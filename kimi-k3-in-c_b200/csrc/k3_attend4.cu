@@ -51,13 +51,13 @@
 // instructions are the largest part and the shared memory (74 KB written, then read once by
 // S and once by O^T) at least 2600; the tensor pipe is busy a third of the time. 512 + 64, one
 // library call:
-//   64 requests, one token, 16 heads, up to 8192 positions    72 us
-//   16 requests, four tokens, 64 heads, up to 8192 positions 103 us
-//   one request, one token, 64 heads: 1000 positions 21 us, 32768 positions 33 us
+//   64 requests, one token, 16 heads, up to 8192 positions    71 us
+//   16 requests, four tokens, 64 heads, up to 8192 positions 101 us
+//   one request, one token, 64 heads: 1000 positions 19 us, 32768 positions 32 us
 // One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
 // Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
 // that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
-// again), and Q by all 14 warps in one batch (121 us where 103 are).
+// again), and Q by all 14 warps in one batch (121 us where one batch of three rows a warp gave 103).
 #include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"
@@ -121,11 +121,10 @@ struct Req {
     int first, n, kvl, items, tiles;
 };
 
-__device__ __forceinline__ Req request(const Args &a, int b)
+__device__ __forceinline__ Req request(const Args &a, int b, int r0, int r1, int kvl)
 {
     Req r;
-    const int r0 = a.row_start[b], r1 = a.row_start[b + 1];
-    int n = r1 - r0, kvl = a.kv_len[b];
+    int n = r1 - r0;
     const int cap = a.max_pages * a.d.page;
     if (r0 < 0 || n < 0 || r1 > a.N || kvl < 0 || kvl > cap) {
         k3_raise_at(K3D_EBOUND, K3_SITE_CACHE4, b, r1, kvl);
@@ -138,6 +137,11 @@ __device__ __forceinline__ Req request(const Args &a, int b)
     r.items = a.hc > 1 ? n * a.hc : (int)((uint32_t)(n + a.per - 1) / (uint32_t)a.per);
     r.tiles = max(1, (kvl + kT - 1) / kT);
     return r;
+}
+
+__device__ __forceinline__ Req request(const Args &a, int b)
+{
+    return request(a, b, a.row_start[b], a.row_start[b + 1], a.kv_len[b]);
 }
 
 // The piece of an item that a CTA works on, and the rows of it.
@@ -704,20 +708,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     pdl_trigger();
 
     // ---- this CTA's units: the requests' totals, then the request that holds the first unit. Up
-    // to 32 requests every warp does it for itself, a request to a lane; more are dealt out over
-    // the block, which meets three times (2 us with one request, of a call's 20).
+    // to 64 requests every warp does it for itself, two requests to a lane; more are dealt out over
+    // the block, which meets three times (1 us more with one request, of a call's 20).
     Cursor cur;
     cur.b = 0; cur.pre = 0;
-    cur.r = Req{0, 0, 0, 0, 1};
+    const Req none = {0, 0, 0, 0, 1};
+    cur.r = none;
     const int c = blockIdx.x;
-    const bool few = a.B <= 32;
-    const int per = few ? 1 : (a.B + kThreads - 1) / kThreads, me = few ? lane : tid;
+    const bool few = a.B <= 64;
+    const int per = few ? 2 : (a.B + kThreads - 1) / kThreads, me = few ? lane : tid;
     const int rb0 = min(a.B, me * per), rb1 = min(a.B, rb0 + per);
     long long mine = 0;
-    Req r0 = cur.r;
-    for (int b = rb0; b < rb1; b++) {
-        r0 = request(a, b);
-        mine += (long long)r0.items * (r0.tiles + kStart);
+    Req lo = none, hi = none;
+    if (few) {
+        if (rb0 < rb1) {
+            const int2 k = make_int2(a.kv_len[rb0], a.kv_len[rb1 - 1]);
+            const int x = a.row_start[rb0], y = a.row_start[rb0 + 1], z = a.row_start[rb1];
+            lo = request(a, rb0, x, y, k.x);
+            if (rb1 - rb0 > 1) hi = request(a, rb0 + 1, y, z, k.y);
+        }
+        mine = (long long)lo.items * (lo.tiles + kStart) + (long long)hi.items * (hi.tiles + kStart);
+    } else {
+        for (int b = rb0; b < rb1; b++) {
+            const Req r = request(a, b);
+            mine += (long long)r.items * (r.tiles + kStart);
+        }
     }
     long long incl = mine;
 #pragma unroll
@@ -753,18 +768,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     };
     if (few) {
         if (cut0 < cut1) {
-            const unsigned at0 = __ballot_sync(0xffffffffu, incl > cut0), at1 = __ballot_sync(0xffffffffu, incl > cut1);
-            const int l0 = __ffs(at0) - 1, l1 = at1 ? __ffs(at1) - 1 : 0;
-            cur.b = l0;
-            cur.pre = __shfl_sync(0xffffffffu, before, l0);
-            cur.r.first = __shfl_sync(0xffffffffu, r0.first, l0);
-            cur.r.n = __shfl_sync(0xffffffffu, r0.n, l0);
-            cur.r.kvl = __shfl_sync(0xffffffffu, r0.kvl, l0);
-            cur.r.items = __shfl_sync(0xffffffffu, r0.items, l0);
-            cur.r.tiles = __shfl_sync(0xffffffffu, r0.tiles, l0);
+            auto holds = [&](int cut, int &b, int &pre, Req &r) {
+                const unsigned m = __ballot_sync(0xffffffffu, incl > cut);
+                const int l = m ? __ffs(m) - 1 : 0, units = lo.items * (lo.tiles + kStart);
+                const bool second = cut >= before + units;
+                const Req &mine = second ? hi : lo;
+                b = 2 * l + __shfl_sync(0xffffffffu, second ? 1 : 0, l);
+                pre = __shfl_sync(0xffffffffu, before + (second ? units : 0), l);
+                r.first = __shfl_sync(0xffffffffu, mine.first, l);
+                r.n = __shfl_sync(0xffffffffu, mine.n, l);
+                r.kvl = __shfl_sync(0xffffffffu, mine.kvl, l);
+                r.items = __shfl_sync(0xffffffffu, mine.items, l);
+                r.tiles = __shfl_sync(0xffffffffu, mine.tiles, l);
+                return m != 0;
+            };
+            int b1, pre1;
+            Req r1;
+            holds(cut0, cur.b, cur.pre, cur.r);
             cur.u = moved_cut(cut0, cur.pre, cur.r.tiles);
-            const int pre1 = __shfl_sync(0xffffffffu, before, l1), tiles1 = __shfl_sync(0xffffffffu, r0.tiles, l1);
-            if (at1) cur.u1 = moved_cut(cut1, pre1, tiles1);
+            if (holds(cut1, b1, pre1, r1)) cur.u1 = moved_cut(cut1, pre1, r1.tiles);
         }
     } else {
         if (tid == 0) s_cur[7] = cut0, s_cur[8] = cut1;

@@ -295,6 +295,21 @@ def test_attend_many_ragged_requests(k3):
     B.compare(got, q, 16, BF16, BF16, 0.07)
 
 
+@pytest.mark.parametrize("B", [2, 31, 32, 33, 63, 64, 65, 449, 900])
+def test_attend_batch_sizes(k3, B):
+    """Some requests without rows, some without positions, one far longer than the others."""
+    g = np.random.default_rng(B)
+    reqs = [(int(g.integers(0, 90)), int(g.integers(0, 3))) for _ in range(B)]
+    reqs = [(max(k, n), n) for k, n in reqs]
+    reqs[B // 2] = (4000, 1)
+    reqs[-1] = (70, 2)
+    b = Batch(k3, 128, 16, 16, reqs, seed=B)
+    n = int(b.start[-1])
+    q = b.queries(24, n, 1.0, BF16)
+    got = b.call(q, 24, n, BF16, F32, 0.07)
+    b.compare(got, q, 24, BF16, F32, 0.07)
+
+
 def test_attend_pages_outside_the_pool(k3):
     """They raise the device error and count as not there."""
     B = Batch(k3, 512, 64, 64, [(200, 1)], seed=9)
