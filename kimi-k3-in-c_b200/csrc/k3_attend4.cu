@@ -1130,15 +1130,94 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
 // threads, so that the pieces, 131 KB each, are read by the whole card; many get blocks of 256
 // threads that lie beside each other on an SM.
 constexpr int kMergeMax = 512;            // threads
+constexpr int kFew = 8;                   // pieces of an item whose weights are held for all rows
 constexpr int kMaxGrid = 512;             // CTAs of k_attend4 (one per SM)
 
-__global__ void __launch_bounds__(kMergeMax, 2) k_attend4_merge(const Args a, int grid, int nrg)
+// a piece that saw nothing has no weight
+__device__ __forceinline__ float weigh(float x, float top, float sum)
+{
+    return x == __int_as_float(0xff800000) && sum == 0.f ? 0.f : exp2f(x - top);
+}
+
+struct Few {
+    int2 rows;                            // the item's first row and how many
+    size_t first;                         // the first piece's slot
+    int c, np, lat;
+    int rg_end, rg0, hop;                 // this thread's row groups
+};
+
+// Up to kFew pieces: the weights of all rows at once, a row to a thread; then a row group after
+// the other, with nothing to wait for but its pieces.
+__device__ __forceinline__ void merge_few(const Args &a, const Few &f, float *w, float4 *s_inv4)   // w: [kFew][64]
+{
+    const int tid = threadIdx.x, odd = tid & 1, kv = a.d.kv;
+    auto slot = [&](int k) { return k == 0 ? f.first : (size_t)(f.c - 1 + k) * 2; };
+    if (tid < f.rows.y) {
+        float2 v[kFew];
+        float M = __int_as_float(0xff800000), l = 0.f;
+#pragma unroll
+        for (int k = 0; k < kFew; k++)
+            if (k < f.np) v[k] = a.ml[slot(k) * kR + tid];
+#pragma unroll
+        for (int k = 0; k < kFew; k++)
+            if (k < f.np) M = fmaxf(M, v[k].x);
+#pragma unroll
+        for (int k = 0; k < kFew; k++)
+            if (k < f.np) {
+                const float x = weigh(v[k].x, M, v[k].y);
+                w[k * kR + tid] = x;
+                l = fmaf(x, v[k].y, l);
+            }
+        reinterpret_cast<float *>(s_inv4)[tid] = l == 0.f ? 0.f : kUnitF / l;
+    }
+    __syncthreads();
+    const float4 *src = reinterpret_cast<const float4 *>(a.part) + (size_t)(f.lat >> 5) * 512 + (f.lat & 31);
+    const size_t step = (size_t)(kv / 32) * 512;
+    for (int g = f.rg0; g < f.rg_end; g += f.hop) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < f.np; k0 += 4) {
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = k0 + k < f.np ? src[slot(k0 + k) * step + g * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (k0 + k >= f.np) break;
+                const float4 x = *reinterpret_cast<const float4 *>(w + (k0 + k) * kR + g * 4);
+                // without weight nothing is added, whatever the piece holds
+                acc[0] = x.x != 0.f ? fmaf(o[k].x, x.x, acc[0]) : acc[0];
+                acc[1] = x.y != 0.f ? fmaf(o[k].y, x.y, acc[1]) : acc[1];
+                acc[2] = x.z != 0.f ? fmaf(o[k].z, x.z, acc[2]) : acc[2];
+                acc[3] = x.w != 0.f ? fmaf(o[k].w, x.w, acc[3]) : acc[3];
+            }
+        }
+        const float4 inv = s_inv4[g];
+        const float u[4] = {inv.x, inv.y, inv.z, inv.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = u[i] == 0.f ? 0.f : acc[i] * u[i];
+        // neighbouring lanes trade, so that each writes a pair of latents of two rows
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? acc[i] : acc[i + 2], 1);
+            const float x = odd ? got : acc[i], y = odd ? acc[i + 2] : got;
+            const int r = g * 4 + i + 2 * odd;
+            if (r < f.rows.y) {
+                const size_t at = (size_t)(f.rows.x + r) * kv + (f.lat & ~1);
+                if (a.out_f32) *reinterpret_cast<float2 *>((float *)a.out + at) = make_float2(x, y);
+                else *reinterpret_cast<uint32_t *>((uint16_t *)a.out + at) = bf16x2(x, y);
+            }
+        }
+    }
+}
+
+template <bool FEW>
+__global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_merge(const Args a, int grid, int nrg)
 {
     __shared__ int s_u0[kMaxGrid + 1], s_begin[kMaxGrid + 1], s_end[kMaxGrid + 1];
     __shared__ int2 s_rows[kMaxGrid + 1];
     __shared__ int s_cnt[kMergeMax / 32], s_c;
     __shared__ float4 s_w[kMaxGrid + 1];               // a piece's weight for four rows
     __shared__ float4 s_red[2][kMergeMax / 32], s_acc[kMergeMax];
+    __shared__ float4 s_inv4[kR / 4];                 // 1 / sum of a row
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
@@ -1181,6 +1260,11 @@ __global__ void __launch_bounds__(kMergeMax, 2) k_attend4_merge(const Args a, in
     const float NEG = __int_as_float(0xff800000);
     const int kv = a.d.kv, share = kv / gridDim.z, ways = blockDim.x / share;
     const int lat = blockIdx.z * share + tid % share, way = tid / share;
+    if (FEW && np <= kFew) {
+        merge_few(a, Few{rw, first, c, np, lat, way < ways ? (rw.y + 3) / 4 : 0, (int)blockIdx.y * ways + way, (int)gridDim.y * ways},
+                  reinterpret_cast<float *>(s_w), s_inv4);
+        return;
+    }
     for (int rg = blockIdx.y; rg < nrg && rg * 4 < rw.y; rg += gridDim.y) {
         const float4 *src = reinterpret_cast<const float4 *>(a.part) + ((size_t)(lat >> 5) * 16 + rg) * 32 + (lat & 31);
         const size_t step = (size_t)(kv / 32) * 512;
@@ -1210,8 +1294,6 @@ __global__ void __launch_bounds__(kMergeMax, 2) k_attend4_merge(const Args a, in
             const float4 t = s_red[0][i];
             M = make_float4(fmaxf(M.x, t.x), fmaxf(M.y, t.y), fmaxf(M.z, t.z), fmaxf(M.w, t.w));
         }
-        // a piece that saw nothing has no weight
-        auto weigh = [&](float x, float top, float sum) { return x == NEG && sum == 0.f ? 0.f : exp2f(x - top); };
         for (int k = tid; k < np; k += blockDim.x) {
             float4 m, s;
             ml4(k, m, s);
@@ -1366,11 +1448,21 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
         // latents down to 64 while that leaves SMs without a block
         const long long rows = ((long long)N + B - 1) / B * H;
         const int most = (H < at4::kR ? at4::kR / H * H : at4::kR) + 3;
-        const int nrg = most / 4, y = (int)(rows < 4LL * nrg ? (rows + 3) / 4 : nrg);
+        const int nrg = most / 4;
+        int y = (int)(rows < 4LL * nrg ? (rows + 3) / 4 : nrg);
         int z = (c->kv_lora + 255) / 256, threads = 256;
-        while (c->kv_lora % (z * 2) == 0 && c->kv_lora / (z * 2) >= 64 && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
-        if ((long long)cuts * y * z <= 2 * grid) threads = 512;
-        launch_pdl(at4::k_attend4_merge, dim3(cuts, y, z), dim3(threads), 0, stream(), a, grid, nrg);
+        // Items that are cut in a few pieces on average: one wave of blocks that go through their
+        // row groups without meeting (64 items: 21 us with a block for each group, 11 so).
+        const bool few = cuts * at4::kFew >= grid;
+        if (few) {
+            const int wave = 5 * grid / (cuts * z);
+            y = y < wave ? y : wave > 1 ? wave : 1;
+        } else {
+            while (c->kv_lora % (z * 2) == 0 && c->kv_lora / (z * 2) >= 64 && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
+            if ((long long)cuts * y * z <= 2 * grid) threads = 512;
+        }
+        launch_pdl(few ? at4::k_attend4_merge<true> : at4::k_attend4_merge<false>, dim3(cuts, y, z), dim3(threads), 0, stream(),
+                   a, grid, nrg);
         note_launch();
         K3_TRY(check_launch("mla attend4 merge"));
     }
