@@ -1322,17 +1322,16 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 if (way + i * ways < np) add(way + i * ways, ahead[i]);
-            int k = way + 4 * ways;
 #pragma unroll 1
-            for (; k + 3 * ways < np; k += 4 * ways) {
+            for (int k = way + 4 * ways; k < np; k += 4 * ways) {
                 float4 o[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = src[slot(k + i * ways) * step];
+                for (int i = 0; i < 4; i++)
+                    o[i] = k + i * ways < np ? src[slot(k + i * ways) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < 4; i++) add(k + i * ways, o[i]);
+                for (int i = 0; i < 4; i++)
+                    if (k + i * ways < np) add(k + i * ways, o[i]);
             }
-#pragma unroll 1
-            for (; k < np; k += ways) add(k, src[slot(k) * step]);
         }
         if (way > 0 && way < ways) s_acc[tid] = acc;
         __syncthreads();
@@ -1445,7 +1444,7 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
     const int cuts = (int)(items < grid - 1 ? items : grid - 1);
     if (cuts > 0) {
         // row groups by the average rows of a request (more are looped over), and shares of the
-        // latents down to 64 while that leaves SMs without a block
+        // latents while they leave SMs without a block
         const long long rows = ((long long)N + B - 1) / B * H;
         const int most = (H < at4::kR ? at4::kR / H * H : at4::kR) + 3;
         const int nrg = most / 4;
@@ -1458,7 +1457,10 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
             const int wave = 5 * grid / (cuts * z);
             y = y < wave ? y : wave > 1 ? wave : 1;
         } else {
-            while (c->kv_lora % (z * 2) == 0 && c->kv_lora / (z * 2) >= 64 && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
+            // shares of 32 latents where an item may have more than 32 pieces (32768 positions:
+            // 32 us with shares of 64, 30.3 with 32), else of 64 (1000 positions: 19.2 and 19.7)
+            const int least = grid > 32 && (long long)max_pages * c->page > 32 * at4::kT ? 32 : 64;
+            while (c->kv_lora % (z * 2) == 0 && c->kv_lora / (z * 2) >= least && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
             if ((long long)cuts * y * z <= 2 * grid) threads = 512;
         }
         launch_pdl(few ? at4::k_attend4_merge<true> : at4::k_attend4_merge<false>, dim3(cuts, y, z), dim3(threads), 0, stream(),
