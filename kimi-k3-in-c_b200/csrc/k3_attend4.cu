@@ -960,106 +960,113 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             if (!dead && !wait_all(b_qfull, item & 1, abort, K3_SITE_CACHE4, 7, item)) dead = true;
             item++;
             const int NR = (s.rows + 15) & ~15;
+            const bool busy = 16 * w < s.rows;            // a warp without rows only keeps in step
             const float fa = score_factor(a, rexp[ra]), fb = score_factor(a, rexp[rb]);
             const int la = sees(a, s, ra), lb = sees(a, s, rb);
             const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
                 const int buf = g & 1;
-                if (!dead && !(wait_all(b_kfull + 8 * (buf * 2 + pieces<NB>() - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
-                               wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
-                    dead = true;
-                tc_after();
-                float v[32];
-                ld_s(lanes + (uint32_t)(buf * kT), v);
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_sfree + 8 * buf);
-                const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
-                const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
-                const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
                 float ca = 1.f, cb = 1.f;
-                // moves the references to a tile's maxima; a row's accumulator changes only if
-                // it held something
-                auto move = [&](float xa, float xb) {
-                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
-                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
-                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
-                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
-                    if (ma == NEG) ma = xa;
-                    else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
-                    if (mb == NEG) mb = xb;
-                    else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
-                };
                 uint32_t pa[8], pb[8];
-                if (plain) {
-                    // every row sees the whole tile, no residuals: the product's maximum is the
-                    // score's, and the sum adds what P is rounded from
-                    float xa = fmaxf(v[0], v[1]), xb = fmaxf(v[2], v[3]);
+                if (busy) {
+                    if (!dead && !(wait_all(b_kfull + 8 * (buf * 2 + pieces<NB>() - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
+                                   wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
+                        dead = true;
+                    tc_after();
+                    float v[32];
+                    ld_s(lanes + (uint32_t)(buf * kT), v);
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b_sfree + 8 * buf);
+                    const int4 k0 = *reinterpret_cast<const int4 *>(kplain + buf * 8);
+                    const int4 k1 = *reinterpret_cast<const int4 *>(kplain + buf * 8 + 4);
+                    const bool plain = (k0.x & k0.y & k0.z & k0.w & k1.x & k1.y & k1.z & k1.w) && t * kT + kT <= low;
+                    // moves the references to a tile's maxima; a row's accumulator changes only if
+                    // it held something
+                    auto move = [&](float xa, float xb) {
+                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 1));
+                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 1));
+                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, 2));
+                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, 2));
+                        if (ma == NEG) ma = xa;
+                        else if (xa > ma + kStep) { ca = ex2(ma - xa); suma *= ca; ma = xa; }
+                        if (mb == NEG) mb = xb;
+                        else if (xb > mb + kStep) { cb = ex2(mb - xb); sumb *= cb; mb = xb; }
+                    };
+                    if (plain) {
+                        // every row sees the whole tile, no residuals: the product's maximum is the
+                        // score's, and the sum adds what P is rounded from
+                        float xa = fmaxf(v[0], v[1]), xb = fmaxf(v[2], v[3]);
 #pragma unroll
-                    for (int i = 1; i < 8; i++) {
-                        xa = fmaxf(xa, fmaxf(v[4 * i], v[4 * i + 1]));
-                        xb = fmaxf(xb, fmaxf(v[4 * i + 2], v[4 * i + 3]));
-                    }
-                    move(xa * fa, xb * fb);
-                    const float na = kLift - (ma == NEG ? 0.f : ma), nb = kLift - (mb == NEG ? 0.f : mb);
-                    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+                        for (int i = 1; i < 8; i++) {
+                            xa = fmaxf(xa, fmaxf(v[4 * i], v[4 * i + 1]));
+                            xb = fmaxf(xb, fmaxf(v[4 * i + 2], v[4 * i + 3]));
+                        }
+                        move(xa * fa, xb * fb);
+                        const float na = kLift - (ma == NEG ? 0.f : ma), nb = kLift - (mb == NEG ? 0.f : mb);
+                        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float p0 = ex2(fmaf(v[4 * i], fa, na)), p1 = ex2(fmaf(v[4 * i + 1], fa, na));
-                        const float p2 = ex2(fmaf(v[4 * i + 2], fb, nb)), p3 = ex2(fmaf(v[4 * i + 3], fb, nb));
-                        s0 += p0; s1 += p1; s2 += p2; s3 += p3;
-                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
-                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
-                    }
-                    suma += s0 + s1;
-                    sumb += s2 + s3;
-                } else {
-                    const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
-                    float xa = NEG, xb = NEG;
-                    float kr[16];
+                        for (int i = 0; i < 8; i++) {
+                            const float p0 = ex2(fmaf(v[4 * i], fa, na)), p1 = ex2(fmaf(v[4 * i + 1], fa, na));
+                            const float p2 = ex2(fmaf(v[4 * i + 2], fb, nb)), p3 = ex2(fmaf(v[4 * i + 3], fb, nb));
+                            s0 += p0; s1 += p1; s2 += p2; s3 += p3;
+                            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                            pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                            pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                        }
+                        suma += s0 + s1;
+                        sumb += s2 + s3;
+                    } else {
+                        const float2 *ki = reinterpret_cast<const float2 *>(kinfo + buf * kT);
+                        float xa = NEG, xb = NEG;
+                        float kr[16];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float2 k = ki[4 * i + t4];  // residuals of two neighbouring positions
-                        const float u0 = unit(k.x), u1 = unit(k.y);
-                        const int pos = t * kT + 8 * i + 2 * t4;
-                        kr[2 * i] = k.x;
-                        kr[2 * i + 1] = k.y;
-                        const bool h0 = k.x != NEG, h1 = k.y != NEG;
-                        v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
-                        v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
-                        v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
-                        v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
-                        xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
-                        xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
-                    }
-                    move(xa, xb);
-                    const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
+                        for (int i = 0; i < 8; i++) {
+                            const float2 k = ki[4 * i + t4];  // residuals of two neighbouring positions
+                            const float u0 = unit(k.x), u1 = unit(k.y);
+                            const int pos = t * kT + 8 * i + 2 * t4;
+                            kr[2 * i] = k.x;
+                            kr[2 * i + 1] = k.y;
+                            const bool h0 = k.x != NEG, h1 = k.y != NEG;
+                            v[4 * i] = h0 && pos < la ? v[4 * i] * fa * u0 : NEG;
+                            v[4 * i + 1] = h1 && pos + 1 < la ? v[4 * i + 1] * fa * u1 : NEG;
+                            v[4 * i + 2] = h0 && pos < lb ? v[4 * i + 2] * fb * u0 : NEG;
+                            v[4 * i + 3] = h1 && pos + 1 < lb ? v[4 * i + 3] * fb * u1 : NEG;
+                            xa = fmaxf(xa, fmaxf(v[4 * i] + k.x, v[4 * i + 1] + k.y));
+                            xb = fmaxf(xb, fmaxf(v[4 * i + 2] + k.x, v[4 * i + 3] + k.y));
+                        }
+                        move(xa, xb);
+                        const float na = (ma == NEG ? 0.f : ma) - kLift, nb = (mb == NEG ? 0.f : mb) - kLift;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float r0 = kr[2 * i], r1 = kr[2 * i + 1];
-                        suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
-                        sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
-                        // a masked position is minus infinity whatever its residual is
-                        const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + r0 - na);
-                        const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + r1 - na);
-                        const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + r0 - nb);
-                        const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + r1 - nb);
-                        const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-                        pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
-                        pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                        for (int i = 0; i < 8; i++) {
+                            const float r0 = kr[2 * i], r1 = kr[2 * i + 1];
+                            suma += ex2(v[4 * i] - na) + ex2(v[4 * i + 1] - na);
+                            sumb += ex2(v[4 * i + 2] - nb) + ex2(v[4 * i + 3] - nb);
+                            // a masked position is minus infinity whatever its residual is
+                            const float p0 = v[4 * i] == NEG ? 0.f : ex2(v[4 * i] + r0 - na);
+                            const float p1 = v[4 * i + 1] == NEG ? 0.f : ex2(v[4 * i + 1] + r1 - na);
+                            const float p2 = v[4 * i + 2] == NEG ? 0.f : ex2(v[4 * i + 2] + r0 - nb);
+                            const float p3 = v[4 * i + 3] == NEG ? 0.f : ex2(v[4 * i + 3] + r1 - nb);
+                            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+                            pa[i] = *reinterpret_cast<const uint32_t *>(&h0);
+                            pb[i] = *reinterpret_cast<const uint32_t *>(&h1);
+                        }
                     }
+                } else if (lane == 0) {
+                    mbar_arrive(b_sfree + 8 * buf);
                 }
                 const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
                 if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
                 // O(t - 1) has been added: P may be written, and the accumulator rescaled
                 if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
                 tc_after();
+                if (busy) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
+                    for (int i = 0; i < 8; i++) {
+                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
+                    }
                 }
                 if (moved && t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
                 if (!moved && t4 == 0) { rowf[ra] = 1.f; rowf[rb] = 1.f; }
