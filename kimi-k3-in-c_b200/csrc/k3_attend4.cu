@@ -453,13 +453,14 @@ __device__ __forceinline__ void widen(uint2 lo, uint2 hi, uint2 scale, uint32_t 
 // ------------------------------------------------------------------------------- Q ----
 // Rows warp, warp + 12, ... of the item: fp16 in units of 2^(e - 14), e the row's exponent (its
 // largest value in [2^13, 2^14)), which the softmax takes into its factor. Rows behind the last
-// are zeros that see everything: they cost no case of their own.
+// up to a multiple of 16 are zeros that see everything: they cost no case of their own. What lies
+// behind them reaches rows of S only that nobody reads.
 template <bool F32>
 __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_t sq, int *rexp, int warp, int lane)
 {
     constexpr int RB = F32 ? 1 : 3;                       // rows in flight (36 registers or 24)
-    const int W = a.d.kv + a.d.rope, chunks = W / 8;
-    for (int r0 = warp; r0 < kR; r0 += 12 * RB) {
+    const int W = a.d.kv + a.d.rope, chunks = W / 8, nr = (s.rows + 15) & ~15;
+    for (int r0 = warp; r0 < nr; r0 += 12 * RB) {
         uint4 raw[RB][3][F32 ? 2 : 1];
 #pragma unroll
         for (int i = 0; i < RB; i++) {
@@ -477,7 +478,7 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
 #pragma unroll
         for (int i = 0; i < RB; i++) {
             const int r = r0 + 12 * i;
-            if (r >= kR) break;
+            if (r >= nr) break;
             auto value = [&](int c, float v[8]) {
                 const uint4 x = raw[i][c][0], y = raw[i][c][F32 ? 1 : 0];
                 const uint32_t u[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
