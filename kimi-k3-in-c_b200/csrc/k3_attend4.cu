@@ -44,16 +44,17 @@
 // warps 8-11 do the softmax and the rescaling; these 12 load Q and write the results; warp
 // 12 issues S, warp 13 O^T. A tile is handed over in pieces of 256 latents: O(t) frees a piece
 // of the buffer, the widening of tile t + 2 fills it while O(t) goes on, and S(t + 2) follows
-// it, so that the softmax of tile t + 1 has the length of O(t) and S(t + 2) to run in. Every
-// wait is bounded (k3_bulk.cuh).
+// it, so that the softmax of tile t + 1 has the length of O(t) and S(t + 2) to run in. Up to 32
+// rows P is held for two tiles in turn, so that it is written while O(t - 1) runs (16 heads: 70 ->
+// 68 us). Every wait is bounded (k3_bulk.cuh).
 //
-// BOUND. A tile of 64 positions x 576 values takes about 3200 cycles, of which the widening's
-// instructions are the largest part and the shared memory (74 KB written, then read once by
-// S and once by O^T) at least 2600; the tensor pipe is busy a third of the time. 512 + 64, one
-// library call:
-//   64 requests, one token, 16 heads, up to 8192 positions    71 us
-//   16 requests, four tokens, 64 heads, up to 8192 positions 101 us
-//   one request, one token, 64 heads: 1000 positions 19 us, 32768 positions 32 us
+// BOUND. A tile of 64 positions x 576 values takes about 3600 cycles: its chain (widening 1500, S
+// 2000, softmax 2300, half of O^T 900) goes round two buffers, which with Q fill the shared
+// memory. The tensor pipe needs 1920 of them (32 for an MMA of S, 48 for one of O^T, both bound
+// by what they read from shared memory), the widening's stores 580. 512 + 64, one call:
+//   64 requests, one token, 16 heads, up to 8192 positions    68 us
+//   16 requests, four tokens, 64 heads, up to 8192 positions  94 us
+//   one request, one token, 64 heads: 1000 positions 19 us, 32768 positions 30 us
 // One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
 // Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
 // that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
@@ -69,6 +70,7 @@ using namespace bulk;
 
 constexpr int kT = 64;                    // positions per tile
 constexpr int kR = 64;                    // rows per item
+constexpr int kHalf = kR / 2;             // rows of which P is held for two tiles in turn
 constexpr int kPanel = kT * 128;          // bytes of a panel: 64 rows x 64 fp16
 constexpr int kThreads = 448;
 constexpr int kMaxUnits = 1 << 30;
@@ -929,12 +931,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 if (stop) break;
                 commit(b_qempty, lead);
             } else {
+                const bool two = __any_sync(0xffffffffu, s.rows <= kHalf);
                 const uint32_t id_o = idesc(128, __reduce_max_sync(0xffffffffu, (s.rows + 15) & ~15), 1);
                 for (int i = 0; i < nt; i++) {
                     stop = !wait_all(b_pfull, (g + i) & 1, abort, K3_SITE_CACHE4, 5, g + i);
                     if (stop) break;
                     tc_after();
-                    issue_o<NB>(a.d.rope, sk, sp, b_pv, id_o, g + i, i ? 1u : 0u, lead);
+                    issue_o<NB>(a.d.rope, sk, sp + (two ? (uint32_t)((g + i) & 1) * (kHalf * 128) : 0u), b_pv, id_o, g + i, i ? 1u : 0u, lead);
                 }
                 if (stop) break;
             }
@@ -962,6 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             item++;
             const int NR = (s.rows + 15) & ~15;
             const bool busy = 16 * w < s.rows;            // a warp without rows only keeps in step
+            const bool two = s.rows <= kHalf;             // P has room for two tiles
             const float fa = score_factor(a, rexp[ra]), fb = score_factor(a, rexp[rb]);
             const int la = sees(a, s, ra), lb = sees(a, s, rb);
             const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
@@ -1059,14 +1063,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 }
                 const bool moved = __any_sync(0xffffffffu, ca != 1.f || cb != 1.f);
                 if (lane == 0) flags[buf * 4 + w] = (moved ? 1 : 0) | (dead ? 2 : 0);
-                // O(t - 1) has been added: P may be written, and the accumulator rescaled
-                if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
-                tc_after();
+                // O(t - 1) has been added: P may be written, and the accumulator rescaled. Of two P
+                // this tile's was read by O(t - 2), which the widening of this tile has waited for.
+                auto added = [&] {
+                    if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                    tc_after();
+                };
+                if (!two) added();
+                const uint32_t sp_t = sp + (two ? (uint32_t)buf * (kHalf * 128) : 0u);
                 if (busy) {
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
-                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp_t + swz(ra, i) + 4 * t4), "r"(pa[i]) : "memory");
+                        asm volatile("st.shared.b32 [%0], %1;" :: "r"(sp_t + swz(rb, i) + 4 * t4), "r"(pb[i]) : "memory");
                     }
                 }
                 if (moved && t4 == 0) { rowf[ra] = ca; rowf[rb] = cb; }
@@ -1076,6 +1085,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 const int f = fl.x | fl.y | fl.z | fl.w;
                 if (f & 2) { dead = true; break; }        // the same for all four warps
                 if ((f & 1) && t > s.t0) {
+                    if (two) added();
                     for (int blk = 0; blk < NB; blk++)
                         for (int c0 = 0; c0 < NR; c0 += 16) {
                             float o[16];
