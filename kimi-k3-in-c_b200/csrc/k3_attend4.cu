@@ -8,7 +8,8 @@
 // positions (none: zeros).
 //
 // WORK. The rows of a request are contiguous in q ([N][H] flattened); an item is up to 64 of
-// them (whole tokens when H <= 64, else 64 heads of one token). An item counts one unit for
+// them (whole tokens when H <= 64, else 64 heads of one token), or up to 32 or 16 where few items
+// would leave SMs idle: Q, the result and the merge are then spread. An item counts one unit for
 // each tile of 64 positions and five for its start (Q, the first tile's way through the
 // pipeline and the result take about as long as five tiles, 10 us), the units of all items,
 // item-major, are cut into one contiguous range per CTA, and a cut that falls into an item's
@@ -54,7 +55,7 @@
 // by what they read from shared memory), the widening's stores 580. 512 + 64, one call:
 //   64 requests, one token, 16 heads, up to 8192 positions    68 us
 //   16 requests, four tokens, 64 heads, up to 8192 positions  94 us
-//   one request, one token, 64 heads: 1000 positions 19 us, 32768 positions 30 us
+//   one request, one token, 64 heads: 1000 positions 17.5 us, 32768 positions 31 us
 // One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
 // Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
 // that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
@@ -82,6 +83,12 @@ constexpr int kUnit = -2;                 // the fp16 operand is in units of 2^k
 constexpr int kDown = 14;                 // a row's 2^e is taken into fp16 for kUnit - 14 <= e <= kUnit
 constexpr float kUnitF = 0.25f;
 
+// How requests are cut into items: up to `rows` rows of whole tokens, or of the heads of one.
+struct Split {
+    int rows;
+    int per, hc;                          // tokens of an item (H <= rows), chunks of `rows` heads of a token
+};
+
 struct Args {
     Pool4 d;
     const void *q;
@@ -89,12 +96,13 @@ struct Args {
     const int *table, *row_start, *kv_len;
     int max_pages, B, N, H;
     int q_f32, out_f32;
-    int per, hc;                          // tokens of an item (H <= 64), chunks of 64 heads of a token
+    Split split[3];                       // 64, 32 and 16 rows
+    int splits;                           // how many of them the kernel may choose from
     float inv_h;                          // 1 / H
     float scale;
     float *part;                          // [grid][2][kv / 32][16][32][4]: latent block, row / 4, latent, row % 4
     float2 *ml;                           // [grid][2][64] (max, sum), base 2
-    int4 *info;                           // [grid][2]: {u0, item begin, item end, 0}, {row0, rows, 0, 0}
+    int4 *info;                           // [grid][2]: {u0, item begin, item end, split}, {row0, rows, 0, 0}
 };
 
 // Pieces of 256 latents in which a tile is handed over.
@@ -124,7 +132,12 @@ struct Req {
     int first, n, kvl, items, tiles;
 };
 
-__device__ __forceinline__ Req request(const Args &a, int b, int r0, int r1, int kvl)
+__device__ __forceinline__ int items_of(const Split &sp, int n)
+{
+    return sp.hc > 1 ? n * sp.hc : (int)((uint32_t)(n + sp.per - 1) / (uint32_t)sp.per);
+}
+
+__device__ __forceinline__ Req request(const Args &a, const Split &sp, int b, int r0, int r1, int kvl)
 {
     Req r;
     int n = r1 - r0;
@@ -137,14 +150,14 @@ __device__ __forceinline__ Req request(const Args &a, int b, int r0, int r1, int
     r.first = r0;
     r.n = n;
     r.kvl = kvl;
-    r.items = a.hc > 1 ? n * a.hc : (int)((uint32_t)(n + a.per - 1) / (uint32_t)a.per);
+    r.items = items_of(sp, n);
     r.tiles = max(1, (kvl + kT - 1) / kT);
     return r;
 }
 
-__device__ __forceinline__ Req request(const Args &a, int b)
+__device__ __forceinline__ Req request(const Args &a, const Split &sp, int b)
 {
-    return request(a, b, a.row_start[b], a.row_start[b + 1], a.kv_len[b]);
+    return request(a, sp, b, a.row_start[b], a.row_start[b + 1], a.kv_len[b]);
 }
 
 // The piece of an item that a CTA works on, and the rows of it.
@@ -160,6 +173,7 @@ struct Seg {
 struct Cursor {
     int u, u1, b, pre;
     Req r;
+    int si;                               // which split
 };
 
 __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
@@ -168,7 +182,7 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
     while (c.u >= c.pre + c.r.items * (c.r.tiles + kStart)) {
         c.pre += c.r.items * (c.r.tiles + kStart);
         c.b++;
-        c.r = request(a, c.b);
+        c.r = request(a, a.split[c.si], c.b);
     }
     const int item = (int)((uint32_t)(c.u - c.pre) / (uint32_t)(c.r.tiles + kStart));
     s.b = c.b;
@@ -178,17 +192,18 @@ __device__ __forceinline__ bool next_seg(const Args &a, Cursor &c, Seg &s)
     s.end = s.begin + c.r.tiles + kStart;
     const int first = c.r.first;
     int last;
-    if (a.hc == 1) {
-        s.j0 = item * a.per;
-        const int tok = min(a.per, c.r.n - s.j0);
+    const Split &sp = a.split[c.si];
+    if (sp.hc == 1) {
+        s.j0 = item * sp.per;
+        const int tok = min(sp.per, c.r.n - s.j0);
         s.row0 = (first + s.j0) * a.H;
         s.rows = tok * a.H;
         last = s.j0 + tok - 1;
     } else {
-        s.j0 = last = (int)((uint32_t)item / (uint32_t)a.hc);
-        const int h0 = (item - s.j0 * a.hc) * kR;
+        s.j0 = last = (int)((uint32_t)item / (uint32_t)sp.hc);
+        const int h0 = (item - s.j0 * sp.hc) * sp.rows;
         s.row0 = (first + s.j0) * a.H + h0;
-        s.rows = min(kR, a.H - h0);
+        s.rows = min(sp.rows, a.H - h0);
     }
     const int stop = min(c.u1, s.end);
     const int seen = max(0, c.r.kvl - c.r.n + last + 1);
@@ -554,9 +569,9 @@ __device__ __forceinline__ float score_factor(const Args &a, int e)
 }
 
 // the positions that row r of the item sees
-__device__ __forceinline__ int sees(const Args &a, const Seg &s, int r)
+__device__ __forceinline__ int sees(const Args &a, const Seg &s, bool tokens, int r)
 {
-    const int j = s.j0 + (a.hc == 1 ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
+    const int j = s.j0 + (tokens ? (int)(((float)r + 0.5f) * a.inv_h) : 0);
     return r < s.rows ? max(0, s.kvl - s.n + j + 1) : 0x7fffffff;
 }
 
@@ -659,7 +674,9 @@ __device__ __forceinline__ void issue_o(int rope, uint32_t sk, uint32_t sp, uint
     }
 }
 
-template <int NB>
+// SPLIT: the kernel chooses how many rows an item has (else 64; with the choice in one kernel the
+// large batches took 1 us more).
+template <int NB, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__ Args a)
 {
     extern __shared__ unsigned char smem_raw[];
@@ -718,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     cur.b = 0; cur.pre = 0;
     const Req none = {0, 0, 0, 0, 1};
     cur.r = none;
+    cur.si = 0;
     const int c = blockIdx.x;
     const bool few = a.B <= 64;
     const int per = few ? 2 : (a.B + kThreads - 1) / kThreads, me = few ? lane : tid;
@@ -728,13 +746,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         if (rb0 < rb1) {
             const int2 k = make_int2(a.kv_len[rb0], a.kv_len[rb1 - 1]);
             const int x = a.row_start[rb0], y = a.row_start[rb0 + 1], z = a.row_start[rb1];
-            lo = request(a, rb0, x, y, k.x);
-            if (rb1 - rb0 > 1) hi = request(a, rb0 + 1, y, z, k.y);
+            lo = request(a, a.split[0], rb0, x, y, k.x);
+            if (rb1 - rb0 > 1) hi = request(a, a.split[0], rb0 + 1, y, z, k.y);
+        }
+        // fewer rows make no fewer tiles
+        const bool idle = SPLIT && __reduce_add_sync(0xffffffffu, lo.items * lo.tiles + hi.items * hi.tiles) <= (int)gridDim.x;
+        for (int i = idle ? a.splits - 1 : 0; i > 0; i--) {
+            const Split sp = a.split[i];
+            const int x = items_of(sp, lo.n), y = items_of(sp, hi.n);
+            if (__reduce_add_sync(0xffffffffu, x * lo.tiles + y * hi.tiles) <= (int)gridDim.x) {
+                cur.si = i;
+                lo.items = x;
+                hi.items = y;
+                break;
+            }
         }
         mine = (long long)lo.items * (lo.tiles + kStart) + (long long)hi.items * (hi.tiles + kStart);
     } else {
         for (int b = rb0; b < rb1; b++) {
-            const Req r = request(a, b);
+            const Req r = request(a, a.split[0], b);
             mine += (long long)r.items * (r.tiles + kStart);
         }
     }
@@ -801,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             if (cut0 < cut1 && cut >= before && cut < before + mine) {
                 int pre = before;
                 for (int b = rb0; b < rb1; b++) {
-                    const Req r = request(a, b);
+                    const Req r = request(a, a.split[0], b);
                     const int len = r.tiles + kStart;
                     if (cut < pre + r.items * len) {
                         s_cur[7 + k] = moved_cut(cut, pre, r.tiles);
@@ -828,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     const int u0 = cur.u;
     if (tid == 12 * 32) {
         // an empty range (its cuts moved together) keeps its place in the order
-        int4 i0 = make_int4(c < G ? u0 : 0x7fffffff, -1, -1, 0), i1 = make_int4(0, 0, 0, 0);
+        int4 i0 = make_int4(c < G ? u0 : 0x7fffffff, -1, -1, cur.si), i1 = make_int4(0, 0, 0, 0);
         Cursor t = cur;
         Seg s;
         if (next_seg(a, t, s)) {
@@ -968,7 +998,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             const bool busy = 16 * w < s.rows;            // a warp without rows only keeps in step
             const bool two = s.rows <= kHalf;             // P has room for two tiles
             const float fa = score_factor(a, rexp[ra]), fb = score_factor(a, rexp[rb]);
-            const int la = sees(a, s, ra), lb = sees(a, s, rb);
+            const bool tokens = a.split[cur.si].hc == 1;
+            const int la = sees(a, s, tokens, ra), lb = sees(a, s, tokens, rb);
             const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
@@ -1141,8 +1172,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     }
 }
 
-// The pieces of each cut item, added in CTA order. Block (k, y, z): the k-th cut item (an item
-// is led by the first CTA boundary inside it), its row groups of four y, y + gridDim.y, ...,
+// The pieces of each cut item, added in CTA order. Block (k, y, z): the k-th cut item of 64 rows (an
+// item is led by the first CTA boundary inside it), its row groups of four y, y + gridDim.y, ...,
 // and the z-th share of the latents. Two round trips to memory: the CTAs' info side by side,
 // then the pieces with their maxima and sums. blockDim / share threads take a latent's pieces
 // in turn and meet in shared memory: few cut items (one long request) get many shares and
@@ -1228,12 +1259,12 @@ __device__ __forceinline__ void merge_few(const Args &a, const Few &f, float *w,
     }
 }
 
-template <bool FEW>
+template <bool FEW, bool SPLIT>
 __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_merge(const Args a, int grid, int nrg)
 {
     __shared__ int s_u0[kMaxGrid + 1], s_begin[kMaxGrid + 1], s_end[kMaxGrid + 1];
     __shared__ int2 s_rows[kMaxGrid + 1];
-    __shared__ int s_cnt[kMergeMax / 32], s_c;
+    __shared__ int s_cnt[kMergeMax / 32], s_c, s_m;        // s_m: the split
     __shared__ float4 s_w[kMaxGrid + 1];               // a piece's weight for four rows
     __shared__ float4 s_red[2][kMergeMax / 32], s_acc[kMergeMax];
     __shared__ float4 s_inv4[kR / 4];                 // 1 / sum of a row
@@ -1247,8 +1278,12 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_
         s_begin[i] = x.y;
         s_end[i] = x.z;
         s_rows[i] = make_int2(y.x, y.y);
+        if (SPLIT && i == 0) s_m = x.w;
     }
     __syncthreads();
+    // items of fewer rows: m of them share the blocks that one of 64 rows has
+    const int sh = SPLIT ? s_m : 0, m = 1 << sh, part = blockIdx.y & (m - 1), which = (blockIdx.x << sh) + part;
+    const int y0 = blockIdx.y >> sh, ny = (gridDim.y - part + m - 1) >> sh;
     int before = 0;
     for (int i0 = 0; i0 < grid; i0 += blockDim.x) {    // once, but for cards of more SMs than threads
         const int i = i0 + tid;
@@ -1261,7 +1296,7 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_
             if (k < warp) rank += s_cnt[k];
             before += s_cnt[k];
         }
-        if (leads && rank == (int)blockIdx.x) s_c = i;
+        if (leads && rank == which) s_c = i;
         __syncthreads();
     }
     const int c = s_c;
@@ -1280,11 +1315,11 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_
     const int kv = a.d.kv, share = kv / gridDim.z, ways = blockDim.x / share;
     const int lat = blockIdx.z * share + tid % share, way = tid / share;
     if (FEW && np <= kFew) {
-        merge_few(a, Few{rw, first, c, np, lat, way < ways ? (rw.y + 3) / 4 : 0, (int)blockIdx.y * ways + way, (int)gridDim.y * ways},
+        merge_few(a, Few{rw, first, c, np, lat, way < ways ? (rw.y + 3) / 4 : 0, y0 * ways + way, ny * ways},
                   reinterpret_cast<float *>(s_w), s_inv4);
         return;
     }
-    for (int rg = blockIdx.y; rg < nrg && rg * 4 < rw.y; rg += gridDim.y) {
+    for (int rg = y0; rg < nrg && rg * 4 < rw.y; rg += ny) {
         const float4 *src = reinterpret_cast<const float4 *>(a.part) + ((size_t)(lat >> 5) * 16 + rg) * 32 + (lat & 31);
         const size_t step = (size_t)(kv / 32) * 512;
         // the first pieces are on their way before their weights are known
@@ -1379,6 +1414,10 @@ static int grid_size()
     return n < kMaxGrid ? n : kMaxGrid;
 }
 
+static Split split(int H, int rows) { return {rows, H <= rows ? rows / H : 1, (H + rows - 1) / rows}; }
+
+static long long most_items(int N, int H, int rows) { return (long long)N * ((H + rows - 1) / rows); }
+
 static size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 struct Ws {
@@ -1396,15 +1435,21 @@ static Ws ws_layout(int kv)
     return w;
 }
 
-template <int NB>
-static cudaError_t launch(const Args &a, int grid, size_t smem, cudaStream_t st)
+template <int NB, bool SPLIT>
+static cudaError_t launch_as(const Args &a, int grid, size_t smem, cudaStream_t st)
 {
     static unsigned long long init = 0;   // one bit per device
     if (!(init & dev_bit())) {
-        allow_smem_max(k_attend4<NB>);
+        allow_smem_max(k_attend4<NB, SPLIT>);
         init |= dev_bit();
     }
-    return launch_pdl(k_attend4<NB>, dim3(grid), dim3(kThreads), smem, st, a);
+    return launch_pdl(k_attend4<NB, SPLIT>, dim3(grid), dim3(kThreads), smem, st, a);
+}
+
+template <int NB>
+static cudaError_t launch(const Args &a, int grid, size_t smem, cudaStream_t st)
+{
+    return a.splits > 1 ? launch_as<NB, true>(a, grid, smem, st) : launch_as<NB, false>(a, grid, smem, st);
 }
 
 }  // namespace at4
@@ -1444,11 +1489,24 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
     K3_TRY(ensure_ctx());
     const at4::Ws w = at4::ws_layout(c->kv_lora);
     char *wb = (char *)ws;
-    const at4::Args a{pool4(c, pool), q, out, table, row_start, kv_len, max_pages, B, N, H,
-                      q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, H <= at4::kR ? at4::kR / H : 1,
-                      (H + at4::kR - 1) / at4::kR, 1.0f / (float)H, scale,
-                      (float *)(wb + w.part), (float2 *)(wb + w.ml), (int4 *)(wb + w.info)};
     const int grid = at4::grid_size();
+    // at most one cut item per CTA boundary, and no more than there are items
+    const long long items = at4::most_items(N, H, at4::kR);
+    const int cuts = (int)(items < grid - 1 ? items : grid - 1);
+    // row groups by the average rows of a request (more are looped over)
+    const long long rows = ((long long)N + B - 1) / B * H;
+    const int most = (H < at4::kR ? at4::kR / H * H : at4::kR) + 3;
+    const int nrg = most / 4;
+    int y = (int)(rows < 4LL * nrg ? (rows + 3) / 4 : nrg);
+    // Fewer rows to an item where the items are so few that the kernel may find idle SMs: the
+    // smallest split whose tiles have a CTA each is taken there (64 heads, 1000 positions: 19.4 us
+    // with items of 64 rows, 17.5 with 16).
+    int splits = 1;
+    while (splits < 3 && B <= 64 && y >= 1 << splits && at4::most_items(N, H, at4::kR >> splits) * 4 <= grid) splits++;
+    const at4::Args a{pool4(c, pool), q, out, table, row_start, kv_len, max_pages, B, N, H,
+                      q_dtype == K3D_DT_F32, out_dtype == K3D_DT_F32, {at4::split(H, 64), at4::split(H, 32), at4::split(H, 16)},
+                      splits, 1.0f / (float)H, scale,
+                      (float *)(wb + w.part), (float2 *)(wb + w.ml), (int4 *)(wb + w.info)};
     const size_t smem = 1024 + at4::smem_layout(c->kv_lora, c->qk_rope).total;
     switch (c->kv_lora / 128) {
     case 1: at4::launch<1>(a, grid, smem, stream()); break;
@@ -1458,16 +1516,7 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
     }
     note_launch();
     K3_TRY(check_launch("mla attend4"));
-    // at most one cut item per CTA boundary, and no more than there are items
-    const long long items = H <= at4::kR ? N : (long long)N * ((H + at4::kR - 1) / at4::kR);
-    const int cuts = (int)(items < grid - 1 ? items : grid - 1);
     if (cuts > 0) {
-        // row groups by the average rows of a request (more are looped over), and shares of the
-        // latents while they leave SMs without a block
-        const long long rows = ((long long)N + B - 1) / B * H;
-        const int most = (H < at4::kR ? at4::kR / H * H : at4::kR) + 3;
-        const int nrg = most / 4;
-        int y = (int)(rows < 4LL * nrg ? (rows + 3) / 4 : nrg);
         int z = (c->kv_lora + 255) / 256, threads = 256;
         // Items that are cut in a few pieces on average: one wave of blocks that go through their
         // row groups without meeting (64 items: 21 us with a block for each group, 11 so).
@@ -1482,8 +1531,9 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
             while (c->kv_lora % (z * 2) == 0 && c->kv_lora / (z * 2) >= least && (long long)cuts * y * z * 2 <= 2 * grid) z *= 2;
             if ((long long)cuts * y * z <= 2 * grid) threads = 512;
         }
-        launch_pdl(few ? at4::k_attend4_merge<true> : at4::k_attend4_merge<false>, dim3(cuts, y, z), dim3(threads), 0, stream(),
-                   a, grid, nrg);
+        launch_pdl(few ? splits > 1 ? at4::k_attend4_merge<true, true> : at4::k_attend4_merge<true, false>
+                       : splits > 1 ? at4::k_attend4_merge<false, true> : at4::k_attend4_merge<false, false>,
+                   dim3(cuts, y, z), dim3(threads), 0, stream(), a, grid, nrg);
         note_launch();
         K3_TRY(check_launch("mla attend4 merge"));
     }

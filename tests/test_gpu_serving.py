@@ -295,6 +295,21 @@ def test_attend_many_ragged_requests(k3):
     B.compare(got, q, 16, BF16, BF16, 0.07)
 
 
+@pytest.mark.parametrize("kv,rope,H,reqs", [
+    (512, 64, 64, [(2000, 1)]), (512, 64, 64, [(3000, 1)]), (512, 64, 64, [(9000, 2), (300, 1)]),   # 16, 32, 64 rows to an item
+    (512, 64, 24, [(1200, 3), (65, 1)]), (512, 64, 24, [(2600, 3), (0, 0), (65, 1)]), (512, 64, 24, [(8000, 5), (65, 1)]),
+    (128, 16, 100, [(600, 1), (1, 1)]), (256, 0, 100, [(1800, 1), (64, 1)]), (128, 16, 100, [(5000, 2), (64, 1)]),
+    (384, 64, 17, [(900, 4)]), (512, 64, 8, [(400, 9), (3, 3)]), (512, 64, 64, [(64, 2)] * 9 + [(1500, 1)]),
+])
+def test_attend_few_items(k3, kv, rope, H, reqs):
+    """Small batches, whose items have fewer rows while that finds idle SMs."""
+    b = Batch(k3, kv, rope, 64, reqs, seed=H + len(reqs))
+    n = int(b.start[-1])
+    q = b.queries(H, n, 1.0, BF16)
+    got = b.call(q, H, n, BF16, F32, 0.07)
+    b.compare(got, q, H, BF16, F32, 0.07)
+
+
 @pytest.mark.parametrize("B", [2, 31, 32, 33, 63, 64, 65, 449, 900])
 def test_attend_batch_sizes(k3, B):
     """Some requests without rows, some without positions, one far longer than the others."""
