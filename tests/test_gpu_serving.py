@@ -300,6 +300,7 @@ def test_attend_many_ragged_requests(k3):
     (512, 64, 24, [(1200, 3), (65, 1)]), (512, 64, 24, [(2600, 3), (0, 0), (65, 1)]), (512, 64, 24, [(8000, 5), (65, 1)]),
     (128, 16, 100, [(600, 1), (1, 1)]), (256, 0, 100, [(1800, 1), (64, 1)]), (128, 16, 100, [(5000, 2), (64, 1)]),
     (384, 64, 17, [(900, 4)]), (512, 64, 8, [(400, 9), (3, 3)]), (512, 64, 64, [(64, 2)] * 9 + [(1500, 1)]),
+    (512, 64, 32, [(64, 2)] * 9 + [(1500, 2)]), (512, 64, 32, [(640, 2)] * 9 + [(1500, 2)]),
 ])
 def test_attend_few_items(k3, kv, rope, H, reqs):
     """Small batches, whose items have fewer rows while that finds idle SMs."""
