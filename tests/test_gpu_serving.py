@@ -725,6 +725,38 @@ def test_serving_step_on_another_stream(k3):
             assert np.array_equal(a[k], b[k]), k
 
 
+@pytest.mark.parametrize("kv,rope", [(128, 16), (512, 64)])
+def test_attend_on_two_streams_at_once(k3, kv, rope):
+    """Two calls with a workspace each, on two streams that do not wait for one another: the same
+    bits as one after the other."""
+    rt = ctypes.CDLL("libcudart.so.12")
+    s = ctypes.c_void_p()
+    batches = [Batch(k3, kv, rope, 64, [(3000, 2), (700, 1)], seed=41), Batch(k3, kv, rope, 64, [(1500, 3)] * 6, seed=42)]
+    sets = []
+    for b in batches:
+        n = int(b.start[-1])
+        q = b.queries(64, n, 1.0, BF16)
+        want = b.call(q, 64, n, BF16, F32, 0.07)
+        nb = k3.k3d_mla_attend4_ws_bytes(b.shape, len(b.reqs), n, 64)
+        sets.append((b, n, DevBuf.from_array(to_bf16(q)), DevBuf(want.nbytes), DevBuf(nb), nb, want))
+    own = k3.k3d_stream()
+    assert rt.cudaStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+    try:
+        for _ in range(8):
+            for (b, n, Q, O, W, nb, _), stream in zip(sets, (own, s)):
+                check(k3.k3d_set_stream(stream))
+                T, R, K = b.bufs
+                check(k3.k3d_mla_attend4(O.ptr, F32, Q.ptr, BF16, b.shape, b.pool.ptr, T.ptr, b.max_pages, R.ptr, K.ptr,
+                                         len(b.reqs), n, 64, 0.07, W.ptr, nb))
+        check(k3.k3d_sync())
+    finally:
+        check(k3.k3d_set_stream(own))
+        check(k3.k3d_sync())
+        rt.cudaStreamDestroy(s)
+    for b, n, Q, O, W, nb, want in sets:
+        assert np.array_equal(O.download(np.float32, want.shape), want)
+
+
 def test_attend_bits_do_not_depend_on_the_run(k3):
     """Splits, merges and launches in one order: the same bits every time."""
     B = Batch(k3, 512, 64, 64, [(5000, 2), (700, 1), (64, 3)], seed=31)
