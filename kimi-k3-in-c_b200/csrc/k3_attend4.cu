@@ -1260,7 +1260,7 @@ __device__ __forceinline__ void merge_few(const Args &a, const Few &f, float *w,
 }
 
 template <bool FEW, bool SPLIT>
-__global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 5 : 2) k_attend4_merge(const Args a, int grid, int nrg)
+__global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 4 : 2) k_attend4_merge(const Args a, int grid, int nrg)
 {
     __shared__ int s_u0[kMaxGrid + 1], s_begin[kMaxGrid + 1], s_end[kMaxGrid + 1];
     __shared__ int2 s_rows[kMaxGrid + 1];
@@ -1522,7 +1522,7 @@ int k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const 
         // row groups without meeting (64 items: 21 us with a block for each group, 11 so).
         const bool few = cuts * at4::kFew >= grid;
         if (few) {
-            const int wave = 5 * grid / (cuts * z);
+            const int wave = 4 * grid / (cuts * z);
             y = y < wave ? y : wave > 1 ? wave : 1;
         } else {
             // shares of 32 latents where an item may have more than 32 pieces (32768 positions:
