@@ -54,7 +54,7 @@
 // memory. The tensor pipe needs 1920 of them (32 for an MMA of S, 48 for one of O^T, both bound
 // by what they read from shared memory), the widening's stores 580. 512 + 64, one call:
 //   64 requests, one token, 16 heads, up to 8192 positions    68 us
-//   16 requests, four tokens, 64 heads, up to 8192 positions  94 us
+//   16 requests, four tokens, 64 heads, up to 8192 positions  93 us
 //   one request, one token, 64 heads: 1000 positions 17.5 us, 32768 positions 31 us
 // One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
 // Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
