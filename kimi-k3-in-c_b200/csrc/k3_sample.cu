@@ -436,13 +436,18 @@ __global__ void __launch_bounds__(kVMax, 2) k_spec_verify(Verify a)
     }
 }
 
-// CTAs to a row: sixteen (more than the portable eight) while the rows take no more than half
-// of the SMs so, eight while they leave SMs idle, else `many`; fewer where a CTA would have
-// less than 2048 elements.
+// CTAs to a row: sixteen (more than the portable eight) while the rows take no more than half of
+// the SMs so, else eight or four while all of them lie on the card at once (two to an SM), else
+// `many`. Each has 4096 elements at least, and 16384 where the rows fill the card anyway, since a
+// CTA's start and exchanges then cost more than its share (300 rows of 10001: 27 us with a least
+// share of 2048, 12 so; of 40000: 36 and 25; 64 rows of 163840: 24.5 us with eight CTAs, 19.3 with
+// four).
 int cluster_of(int rows, int V, int many)
 {
-    int cs = (long long)rows * 32 <= sm_count() ? 16 : (long long)rows * 8 <= 4 * sm_count() ? 8 : many;
-    while (cs > 1 && V < cs * 2048) cs >>= 1;
+    const long long room = 2LL * sm_count();
+    int cs = rows * 64LL <= room ? 16 : rows * 8LL <= room ? 8 : rows * 4LL <= room ? 4 : many;
+    const int least = rows * 4LL > room ? 16384 : 4096;
+    while (cs > 1 && V < (long long)cs * least) cs >>= 1;
     return cs;
 }
 

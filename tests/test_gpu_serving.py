@@ -458,6 +458,15 @@ def test_softmax(k3, rows, V):
     softmax_close(softmax(k3, x, temp, off=1), x, temp)
 
 
+@pytest.mark.parametrize("rows,V", [(36, 33000), (38, 33000), (75, 33001), (160, 17000), (300, 2500), (5, 70000)])
+def test_softmax_row_counts(k3, rows, V):
+    """Sixteen, eight, four or one CTA to a row, greedy rows among them."""
+    g = np.random.default_rng(rows)
+    x = (g.standard_normal((rows, V)) * 4).astype(np.float32)
+    temp = np.where(np.arange(rows) % 3 == 0, 0.0, 0.7).astype(np.float32)
+    softmax_close(softmax(k3, x, temp), x, temp)
+
+
 def test_softmax_greedy_takes_the_first_maximum(k3):
     x = np.zeros((4, 20000), np.float32)
     x[0, [777, 15000]] = 3.0
