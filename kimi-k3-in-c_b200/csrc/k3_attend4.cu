@@ -47,7 +47,8 @@
 // of the buffer, the widening of tile t + 2 fills it while O(t) goes on, and S(t + 2) follows
 // it, so that the softmax of tile t + 1 has the length of O(t) and S(t + 2) to run in. Up to 32
 // rows P is held for two tiles in turn, so that it is written while O(t - 1) runs (16 heads: 70 ->
-// 68 us). Every wait is bounded (k3_bulk.cuh).
+// 68 us). What is held for two tiles has a barrier for each (k3_attend4_order.h); every wait is
+// bounded (k3_bulk.cuh).
 //
 // BOUND. A tile of 64 positions x 576 values takes about 3600 cycles: its chain (widening 1500, S
 // 2000, softmax 2300, half of O^T 900) goes round two buffers, which with Q fill the shared
@@ -61,6 +62,7 @@
 // that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
 // again), Q by all 14 warps in one batch (103 -> 121 us), and Q through a bulk copy into the free
 // tile buffer (68 -> 69.5 us: its conversion takes the time, not its way).
+#include "k3_attend4_order.h"
 #include "k3_bulk.cuh"
 #include "k3_cache4.cuh"
 #include "k3_ops.cuh"
@@ -630,13 +632,13 @@ template <int NB>
 __device__ __forceinline__ bool issue_s(int rope, uint32_t sq, uint32_t sk, uint32_t b_kfull, uint32_t b_sfull,
                                         uint32_t b_sfree, volatile int *abort, int k, uint32_t lead)
 {
-    const int buf = k & 1;
-    if (k >= 2 && !wait_all(b_sfree + 8 * buf, ((k >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 13, k)) return false;
+    const int buf = at4_buf(k);
+    if (k >= 2 && !wait_all(b_sfree + 8 * buf, at4_phase(k - 2), abort, K3_SITE_CACHE4, 13, k)) return false;
     uint32_t da = desc_k(sq), db = desc_k(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel);
     const uint32_t id = idesc(64, kT, 0), d = (uint32_t)(buf * kT);
 #pragma unroll 1
     for (int i = 0; i < NB; i++) {
-        if (!(i & 1) && !wait_all(b_kfull + 8 * (buf * 2 + (i >> 1)), (k >> 1) & 1, abort, K3_SITE_CACHE4, 4, k)) return false;
+        if (!(i & 1) && !wait_all(b_kfull + 8 * (buf * 2 + (i >> 1)), at4_phase(k), abort, K3_SITE_CACHE4, 4, k)) return false;
         tc_after();
 #pragma unroll
         for (int p = 0; p < 2; p++) {
@@ -658,7 +660,7 @@ template <int NB>
 __device__ __forceinline__ void issue_o(int rope, uint32_t sk, uint32_t sp, uint32_t b_pv, uint32_t id, int k, uint32_t accum,
                                         uint32_t lead)
 {
-    const int buf = k & 1;
+    const int buf = at4_buf(k);
     uint32_t da = desc_mn(sk + (uint32_t)buf * (NB * 2 + (rope ? 1 : 0)) * kPanel, kPanel), d = kColO, bar = b_pv + 16 * buf;
     const uint32_t db = desc_k(sp);
 #pragma unroll 1
@@ -693,11 +695,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
     int *flags = reinterpret_cast<int *>(gb + L.row + 2 * kR * 4);      // [2][4]
     const uint32_t b_qfull = base + L.bars, b_qempty = b_qfull + 8;
     // of each tile buffer and 256 latents: widened (kfull), and O^T added (pv, the last of a tile
-    // standing for the tile)
+    // standing for the tile); S, P and "S is read" (sfree) of each buffer
     const uint32_t b_kfull = b_qfull + 16, b_pv = b_kfull + 64, b_sfull = b_pv + 64, b_pfull = b_sfull + 16;
-    const uint32_t b_drain = b_pfull + 8, b_sfree = b_drain + 8;
-    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 192);
-    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 196);
+    const uint32_t b_drain = b_pfull + 16, b_sfree = b_drain + 8;
+    volatile int *abort = reinterpret_cast<volatile int *>(gb + L.bars + 200);
+    uint32_t *tslot = reinterpret_cast<uint32_t *>(gb + L.bars + 204);
     int *kplain = reinterpret_cast<int *>(gb + L.bars + 208);           // [2][8]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -711,6 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
         mbar_init(b_sfull, 1);
         mbar_init(b_sfull + 8, 1);
         mbar_init(b_pfull, 4);
+        mbar_init(b_pfull + 8, 4);
         mbar_init(b_drain, 2);
         mbar_init(b_sfree, 4);
         mbar_init(b_sfree + 8, 4);
@@ -909,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     advance(at, a.d.page);
                     look_up(at, table, s.kvl);
                 }
-                const int buf = g & 1;
+                const int buf = at4_buf(g);
                 const uint32_t tile = sk + (uint32_t)buf * panels * kPanel, up = unit_step(r.e);
                 // the residual; NaN for a row of NaN, minus infinity where there is none
                 const int e = r.e - 127;
@@ -919,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 // as soon as O(g - 2) has used 256 latents of the buffer, this tile's take their place
 #pragma unroll
                 for (int h = 0; h < pieces<NB>(); h++) {
-                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 2 + h), ((g >> 1) - 1) & 1, abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
+                    if (g >= 2 && !wait_all(b_pv + 8 * (buf * 2 + h), at4_phase(g - 2), abort, K3_SITE_CACHE4, 2, g)) { dead = true; break; }
 #pragma unroll
                     for (int i = 2 * h; i < 2 * h + 2 && i < NB; i++)
                         widen(r.lo[i], r.hi[i], r.scale[i], up, tile + 2 * i * kPanel, at0, at1, sel);
@@ -965,10 +968,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 const bool two = __any_sync(0xffffffffu, s.rows <= kHalf);
                 const uint32_t id_o = idesc(128, __reduce_max_sync(0xffffffffu, (s.rows + 15) & ~15), 1);
                 for (int i = 0; i < nt; i++) {
-                    stop = !wait_all(b_pfull, (g + i) & 1, abort, K3_SITE_CACHE4, 5, g + i);
+                    stop = !wait_all(b_pfull + 8 * at4_buf(g + i), at4_phase(g + i), abort, K3_SITE_CACHE4, 5, g + i);
                     if (stop) break;
                     tc_after();
-                    issue_o<NB>(a.d.rope, sk, sp + (two ? (uint32_t)((g + i) & 1) * (kHalf * 128) : 0u), b_pv, id_o, g + i, i ? 1u : 0u, lead);
+                    issue_o<NB>(a.d.rope, sk, sp + (two ? (uint32_t)at4_buf(g + i) * (kHalf * 128) : 0u), b_pv, id_o, g + i, i ? 1u : 0u, lead);
                 }
                 if (stop) break;
             }
@@ -1003,12 +1006,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
             const int low = __reduce_min_sync(0xffffffffu, min(la, lb));   // what every row of the warp sees
             float ma = NEG, mb = NEG, suma = 0.f, sumb = 0.f;
             for (int t = s.t0; t < s.t1; t++, g++) {
-                const int buf = g & 1;
+                const int buf = at4_buf(g);
                 float ca = 1.f, cb = 1.f;
                 uint32_t pa[8], pb[8];
                 if (busy) {
-                    if (!dead && !(wait_all(b_kfull + 8 * (buf * 2 + pieces<NB>() - 1), (g >> 1) & 1, abort, K3_SITE_CACHE4, 8, g) &&
-                                   wait_all(b_sfull + 8 * buf, (g >> 1) & 1, abort, K3_SITE_CACHE4, 9, g)))
+                    if (!dead && !(wait_all(b_kfull + 8 * (buf * 2 + pieces<NB>() - 1), at4_phase(g), abort, K3_SITE_CACHE4, 8, g) &&
+                                   wait_all(b_sfull + 8 * buf, at4_phase(g), abort, K3_SITE_CACHE4, 9, g)))
                         dead = true;
                     tc_after();
                     float v[32];
@@ -1098,7 +1101,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 // O(t - 1) has been added: P may be written, and the accumulator rescaled. Of two P
                 // this tile's was read by O(t - 2), which the widening of this tile has waited for.
                 auto added = [&] {
-                    if (t > s.t0 && !dead && !wait_all(b_pv + 8 * ((buf ^ 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 10, g)) dead = true;
+                    if (t > s.t0 && !dead && !wait_all(b_pv + 8 * (at4_buf(g - 1) * 2 + pieces<NB>() - 1), at4_phase(g - 1), abort, K3_SITE_CACHE4, 10, g)) dead = true;
                     tc_after();
                 };
                 if (!two) added();
@@ -1131,7 +1134,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                 async_fence();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(b_pfull);
+                if (lane == 0) mbar_arrive(b_pfull + 8 * buf);
             }
             // ---- the item's sums
             suma += __shfl_xor_sync(0xffffffffu, suma, 1);
@@ -1149,7 +1152,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
                     a.ml[slot * kR + rb] = make_float2(mb, sumb);
                 }
             }
-            if (any && !dead && !wait_all(b_pv + 8 * (((g - 1) & 1) * 2 + pieces<NB>() - 1), ((g - 1) >> 1) & 1, abort, K3_SITE_CACHE4, 11, g)) dead = true;
+            if (any && !dead && !wait_all(b_pv + 8 * (at4_buf(g - 1) * 2 + pieces<NB>() - 1), at4_phase(g - 1), abort, K3_SITE_CACHE4, 11, g)) dead = true;
             tc_after();
             tc_before();
             named_sync(2, 384);

@@ -791,3 +791,37 @@ def test_attend_lengths_that_do_not_fit(k3):
     assert k3.k3d_sync() == k3cuda.K3D_EDEVICE
     k3.k3d_clear_status()
     assert np.abs(got[:1] - ref.attend(q[:1], B.values[0], 256, 0.07, 1)).max() <= 2.0 ** -6
+
+
+@pytest.mark.parametrize("kv,rope,H", [(128, 0, 16), (512, 64, 16), (256, 32, 32)])
+def test_attend_of_few_rows_beside_other_work(k3, kv, rope, H):
+    """Items of up to 32 rows, whose P is held for two tiles, many tiles each, beside another call on
+    a second stream that takes the memory and the issue slots: the same bits as alone."""
+    rt = ctypes.CDLL("libcudart.so.12")
+    s = ctypes.c_void_p()
+    b = Batch(k3, kv, rope, 64, [(4000, 1)] * 6 + [(900, 1), (3001, 1)], seed=51)
+    n = int(b.start[-1])
+    q = b.queries(H, n, 1.0, BF16)
+    want = b.call(q, H, n, BF16, F32, 0.07)
+    b.compare(want, q, H, BF16, F32, 0.07)
+    nb = k3.k3d_mla_attend4_ws_bytes(b.shape, len(b.reqs), n, H)
+    Q, O, W = DevBuf.from_array(to_bf16(q)), DevBuf(want.nbytes), DevBuf(nb)
+    x = np.zeros((64, 100000), np.float32)
+    X, P = DevBuf.from_array(x), DevBuf(x.nbytes)
+    own = k3.k3d_stream()
+    assert rt.cudaStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+    try:
+        for _ in range(20):
+            check(k3.k3d_set_stream(s))
+            check(k3.k3d_logits_softmax(P.ptr, X.ptr, None, *x.shape))
+            check(k3.k3d_set_stream(own))
+            T, R, K = b.bufs
+            check(k3.k3d_mla_attend4(O.ptr, F32, Q.ptr, BF16, b.shape, b.pool.ptr, T.ptr, b.max_pages, R.ptr, K.ptr,
+                                     len(b.reqs), n, H, 0.07, W.ptr, nb))
+        check(k3.k3d_sync())
+    finally:
+        check(k3.k3d_set_stream(s))
+        check(k3.k3d_sync())
+        check(k3.k3d_set_stream(own))
+        rt.cudaStreamDestroy(s)
+    assert np.array_equal(O.download(np.float32, want.shape), want)
