@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 
 import attend_bound as ab
-from test_gpu_serving import BF16, F32, SHAPES, Batch
+import serving_ref as ref
+from k3cuda import DevBuf, check
+from test_gpu_serving import BF16, F32, SHAPES, Batch, Loop, same_pages, to_bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +67,55 @@ def test_attend_moving_maximum(k3, kv, rope, H, n, gain):
     N = int(B.start[-1])
     q = ab.grid_queries(g, N, H, kv, rope, gain, True)
     held(B, B.call(q, H, N, BF16, F32, 2.0 ** -4), q, 2.0 ** -4, F32, True)
+
+
+class Bf16Loop(Loop):
+    """The serving step with bf16 queries, which the kernel takes as they are."""
+
+    def __init__(self, lib, g, **kw):
+        super().__init__(lib, g, **kw)
+        self.q16 = DevBuf(self.N * self.H * self.w * 2)
+
+    def calls(self):
+        lib, d = self.lib, {k: b.ptr for k, b in self.dev.items()}
+        check(lib.k3d_page_plan(self.pages.p, d["len"], d["new"], self.B, self.N, d["start"], d["kvl"], d["pos"],
+                                d["slots"], d["status"]))
+        check(lib.k3d_cache4_store(self.shape, self.pool.ptr, d["x"], F32, self.w, d["slots"], self.N))
+        check(lib.k3d_mla_attend4(d["o"], F32, self.q16.ptr, BF16, self.shape, self.pool.ptr, self.pages.t.ptr, 12, d["start"],
+                                  d["kvl"], self.B, self.N, self.H, 0.07, self.ws.ptr, self.nws))
+
+
+@pytest.mark.parametrize("H,kv,rope", [(16, 256, 32), (64, 512, 64)])
+def test_serving_steps_position_by_position(k3, H, kv, rope):
+    """plan -> store -> attend over steps that keep some of their drafts, ragged and with a request that
+    brings nothing: every element within the bound, which a position too many or too few leaves."""
+    g = np.random.default_rng(61)
+    L = Bf16Loop(k3, g, B=5, K=3, H=H, kv=kv, rope=rope)
+    lens = np.zeros(L.B, int)
+    known = [(np.zeros((0, L.w)), np.zeros(0, int)) for _ in range(L.B)]
+    for step in range(7):
+        new = [4, 1, 3, 0 if step == 2 else 2, 4]
+        h = L.inputs(lens, new)
+        L.q16.upload(to_bf16(h["q"]))
+        L.calls()
+        check(k3.k3d_sync())
+        code, start, kvl, _, slots = L.host.plan(lens.tolist(), new, L.N)
+        assert code == 0
+        same_pages(L.pages, L.host)
+        o = L.dev["o"].download(np.float32, (L.N, H, kv))
+        fields, value = ref.quantise(h["x"], kv)
+        e = fields[3].astype(int) - 127
+        for b in range(L.B):
+            r = slice(start[b], start[b + 1])
+            v = np.concatenate([known[b][0][:lens[b]], value[r]])
+            x = np.concatenate([known[b][1][:lens[b]], e[r]])
+            known[b] = (v, x)
+            if new[b]:
+                want, tol = ab.bound(h["q"][r], v, x, kv, float(np.float32(0.07)), new[b])
+                assert (np.abs(o[r] - want) <= tol).all(), (step, b)
+                if lens[b] + new[b] > 1:
+                    lost = ab.without(h["q"][r], v, kv, 0.07, new[b], 0)
+                    assert (np.abs(lost - want) > tol).any(), "the bound sees the first position"
+        lens = lens + np.minimum(new, g.integers(1, 4, L.B))          # some of the drafts are kept
+        if step == 4:
+            lens[1] = 0                                               # a request ended, another in its place
