@@ -508,13 +508,16 @@ int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtyp
  * cached positions, its new ones (stored before this call) among them; its row j sees the
  * first kv_len[b] - rows + j + 1 positions, and gets zeros when that is none. Rows from
  * row_start[B] to N are left as they were. table [B][max_pages] as in K3dPages. Scores,
- * softmax and sums are fp32; q is rounded to fp16 in units of its row (exact for bf16) and
- * the softmax weights to fp16. A page id outside the pool, a kv_len above max_pages * page,
- * or a row_start that is not a prefix sum within N raises K3D_EBOUND; such positions count as
- * not there. A call whose tiles of 64 positions, counted for every 64 rows, pass 2^30 raises
- * it too and writes nothing. Weights below about 2^-31 of a row's largest count as 0. N H and
- * max_pages * page are at most 2^30. The workspace belongs to the call until it has run: two
- * calls that may run at the same time (two streams, two graphs) need one each. */
+ * softmax and sums are fp32. Rounded to fp16 are, whatever the types of q and out: q in units of
+ * its row (2^-11 of an fp32 value; exact for bf16 within 2^-29 of the row's largest), the softmax
+ * weights (2^-11), and rotated keys below 2^-16 of rows with -16 <= e < -2, to multiples of 2^-26
+ * (with e below -16: keys below 2^e, to multiples of 2^(e - 10)). A page id outside the pool, a
+ * kv_len above max_pages * page, or a row_start that is not a prefix sum within N raises
+ * K3D_EBOUND; such positions count as not there. A call whose tiles of 64 positions, counted for
+ * every 64 rows, pass 2^30 raises it too and writes nothing. Weights below about 2^-31 of a row's
+ * largest count as 0. N H and max_pages * page are at most 2^30. The workspace belongs to the call
+ * until it has run: two calls that may run at the same time (two streams, two graphs) need one
+ * each. */
 size_t k3d_mla_attend4_ws_bytes(const K3dCache4 *c, int B, int N, int H);
 int    k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const K3dCache4 *c,
                        const void *pool, const int *table, int max_pages, const int *row_start,

@@ -29,12 +29,13 @@
 // O^T rather than O keeps the accumulator of 64 rows in 256 of the 512 columns, which leaves
 // room for two S; O of 64 rows and 512 latents would fill all of them.
 //
-// UNITS. The fp16 operand holds values in units of 2^-2. A stored row is a multiple of 2^-10
-// of its own 2^e, so for -16 <= e <= -2 (largest latent between 0.02 and 672) the step to
-// 2^-2 is exact in fp16. A row outside keeps a residual 2^r in fp32: its scores are
-// multiplied by it, and its weight P carries it into the second product, so that rows of any
-// size stay exact. q is fp16 in units of its row (exact for bf16 within 2^-29 of the row's
-// largest value).
+// UNITS. The fp16 operand holds values in units of 2^-2. A stored row's latents are multiples of
+// 2^-10 of its own 2^e, so for -16 <= e <= -2 (largest latent between 0.02 and 672) their step to
+// 2^-2 is exact in fp16. A row outside keeps a residual 2^r in fp32: its scores are multiplied by
+// it, and its weight P carries it into the second product, so that latents of any size stay exact.
+// The rotated key is any fp16 number of 2^e: for e < -2 its step rounds by at most 2^-25 of the unit
+// 2^(-2 + r), 2^-11 of 2^e at most, where the row's largest value is at least 1344 of them. q is
+// fp16 in units of its row (exact for bf16 within 2^-29 of the row's largest value).
 //
 // SOFTMAX. With a = s log2(e) + r: P = 2^(a - m + 7), rounded to fp16 (half a step is 2^-12
 // on average, an eighth of a bf16 result's), and the sum takes 2^(a - r - m + 7) in fp32. m

@@ -8,8 +8,9 @@
 //   latent  blocks of 16: s = e4m3(max|x| 2^-e / 6), codes e2m1(x 2^-e / s), ties to even
 //   rope    fp16 of x 2^-e
 // Within a row every value is therefore an fp16 number times 2^e: code x scale has at most
-// six significant bits and lies in [2^-10, 2688], so the attention multiplies fp16 operands
-// without a rounding and applies 2^e per key.
+// six significant bits and lies in [2^-10, 2688], so the attention multiplies fp16 latents
+// without a rounding and applies 2^e per key. (Rotated keys far below their row's
+// latents are rounded on the way, k3_attend4.cu.)
 // A page holds `page` rows as four arrays, each 16-byte aligned (page is a multiple of 16):
 //   codes [page][kv/2] | scales [page][kv/16] | rope [page][rope] fp16 | exponents [page]
 #pragma once

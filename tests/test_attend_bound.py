@@ -92,3 +92,32 @@ def test_a_skipped_rescale_is_outside(gain):
     top = s[0].argmax(1)
     for h in range(4):
         assert outside(ab.without(q, v, kv, 2.0 ** -4, n, int(top[h])), want, tol)
+
+
+def test_small_rotated_keys_under_large_latents():
+    """Their rounding is in the bound: without the term, keys that the kernel loses would be outside,
+    and with it a result that drops the rotated part altogether still is."""
+    g = np.random.default_rng(7)
+    kv, rope, L, n = 128, 64, 40, 1
+    x = (g.standard_normal((L, kv + rope)) * 2.0 ** -7).astype(np.float32)
+    x[:, kv:] *= np.float32(2.0 ** -8)
+    q = np.zeros((n, 4, kv + rope), np.float32)
+    q[:, :, kv:] = g.integers(-4, 5, (n, 4, rope)) * 1024.0
+    v, e = values(x, kv)
+    want, tol = ab.bound(q, v, e, kv, 1.0, n)
+    res = e - np.clip(e, -16, -2)
+    assert (e < -2).all()
+    # the rotated keys as the kernel has them, in units of 2^(res - 2)
+    up = np.ldexp(v[:, kv:], -e[:, None]).astype(np.float64)
+    k16 = np.ldexp(up, np.clip(e + 2, -14, 0)[:, None]).astype(np.float16).astype(np.float64)
+    w = v.copy()
+    w[:, kv:] = np.ldexp(k16, (res - 2)[:, None])
+    assert (np.abs(w[:, kv:] - v[:, kv:]) <= np.ldexp(1.0, -27 + res)[:, None]).all() and (w != v).any()
+    s = q[0].astype(np.float64) @ w.T
+    p = np.exp(s - s.max(1, keepdims=True))
+    got = (p / p.sum(1, keepdims=True)) @ v[:, :kv]
+    assert not outside(got[None], want, tol)
+    w[:, kv:] = 0
+    s = q[0].astype(np.float64) @ w.T
+    p = np.exp(s - s.max(1, keepdims=True))
+    assert outside(((p / p.sum(1, keepdims=True)) @ v[:, :kv])[None], want, tol)

@@ -69,6 +69,20 @@ def test_attend_moving_maximum(k3, kv, rope, H, n, gain):
     held(B, B.call(q, H, N, BF16, F32, 2.0 ** -4), q, 2.0 ** -4, F32, True)
 
 
+@pytest.mark.parametrize("H", [64, 16])
+def test_attend_small_rotated_keys_under_large_latents(k3, H):
+    """Queries on the rotated part alone, of keys so small that their way to fp16 rounds them."""
+    kv, rope = 128, 64
+
+    def edit(b, x):
+        x *= np.float32(2.0 ** -7)
+        x[:, kv:] *= np.float32(2.0 ** -8)
+    B = Batch(k3, kv, rope, 64, [(40, 1), (300, 2)], seed=13, spread=0.0, edit=edit)
+    q = np.zeros((3, H, kv + rope), np.float32)
+    q[:, :, kv:] = np.random.default_rng(13).integers(-4, 5, (3, H, rope)) * 1024.0
+    held(B, B.call(q, H, 3, BF16, F32, 1.0), q, 1.0, F32, False)
+
+
 class Bf16Loop(Loop):
     """The serving step with bf16 queries, which the kernel takes as they are."""
 
