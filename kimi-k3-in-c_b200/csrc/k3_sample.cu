@@ -87,10 +87,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
     const float T = temp ? temp[r] : 1.0f;
     const float NEG = __int_as_float(0xff800000), POS = __int_as_float(0x7f800000);
     const bool greedy = !(T > 0.f);
-    const float c = fminf(1.4426950408889634f / T, 3.4028234e38f);   // finite at a subnormal T: 0 c stays 0
+    // 2 log2(e) / T, for differences that are taken in halves, since t - m alone may leave fp32 where
+    // (t - m) / T does not; finite at a subnormal T: 0 c stays 0
+    const float c = fminf(2.885390081777927f / T, 3.4028234e38f);
     constexpr int W = VEC ? 4 : 1, U = VEC ? 10 : 20, nw = kSmThreads / 32;   // values of a load, loads of a step
-    // e^((t - m) / T); minus infinity is 0 at any temperature, an infinite one too
-    auto weigh = [&](float t, float m) { return t > NEG ? ex2((t - m) * c) : 0.f; };
+    // e^((t - 2 h) / T), h half of the largest; minus infinity is 0 at any temperature, an infinite one too
+    auto weigh = [&](float t, float h) { return t > NEG ? ex2(fmaf(t, 0.5f, -h) * c) : 0.f; };
     auto load = [&](float v[U][W], int i0) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
                         if (v[u][k] == top) first = c0 + i0 + u * kSmThreads * W + k;
             }
         } else if (top < POS) {
-            const float ref = top > NEG ? top : 0.f;
+            const float ref = top > NEG ? 0.5f * top : 0.f;
             s *= weigh(m, ref);
 #pragma unroll
             for (int u = 0; u < U; u++)
@@ -147,7 +149,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
         first = __reduce_min_sync(0xffffffffu, m == mc ? first : 0x7fffffff);
         if (lane == 0) red_i[warp] = first;
     } else {
-        s = warp_sum(m > NEG && mc < POS ? s * exp2f((m - mc) * c) : 0.f);
+        s = warp_sum(m > NEG && mc < POS ? s * exp2f((0.5f * m - 0.5f * mc) * c) : 0.f);
         if (lane == 0) red_s[warp] = s;
     }
     __syncthreads();
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
     }
     float S;
     if (M < POS) {
-        S = warp_sum(lane < csize && mk > NEG ? sk * exp2f((mk - M) * c) : 0.f);
+        S = warp_sum(lane < csize && mk > NEG ? sk * exp2f((0.5f * mk - 0.5f * M) * c) : 0.f);
     } else {
         // +inf in the row: its places are counted
         float k = 0.f;
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
         cl_sync();
         S = warp_sum(lane < csize ? cl_ld_f32(&x_n, lane) : 0.f);
     }
-    const float inv = S > 0.f ? 1.0f / S : 0.f, ref = M > NEG ? M : 0.f;
+    const float inv = S > 0.f ? 1.0f / S : 0.f, ref = M > NEG ? 0.5f * M : 0.f;
     for (int i0 = tid * W; i0 < n; i0 += step) {
         float v[U][W];
         load(v, i0);

@@ -506,6 +506,19 @@ def test_softmax_at_the_ends_of_the_temperatures(k3):
     assert (got[:3, 3] == 0.5).all() and (got[:3, 4001] == 0.5).all()
 
 
+@pytest.mark.parametrize("V", [9000, 9001])
+def test_softmax_of_logits_further_apart_than_fp32(k3, V):
+    """x - max passes fp32's largest number where (x - max) / T does not."""
+    g = np.random.default_rng(V)
+    x = (g.standard_normal((5, V)) * 1e38).clip(-3.4e38, 3.4e38).astype(np.float32)
+    x[:, 3], x[:, 700], x[4] = 3.4e38, -3.4e38, np.tile(np.float32([3.4e38, -3.4e38]), V)[:V]
+    x[1, 5::7] = -np.inf
+    temp = np.array([1e38, 3e38, np.inf, 5e37, np.inf], np.float32)
+    got = softmax(k3, x, temp)
+    softmax_close(got, x, temp)
+    assert (np.abs(got[[2, 4]] * V - 1) <= 1e-5).all() and got[0, 700] > 0
+
+
 # ------------------------------------------------------------------------ verification ----
 def verify(lib, target, draft, ids, nd, u, us):
     B, K1, V = target.shape
