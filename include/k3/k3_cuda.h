@@ -506,8 +506,9 @@ int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtyp
  * queries of the new rows, out [N][H][kv_lora] the attended latents, each fp32 or bf16 and
  * 16-byte aligned. Request b owns the rows row_start[b] .. row_start[b + 1] and kv_len[b]
  * cached positions, its new ones (stored before this call) among them; its row j sees the
- * first kv_len[b] - rows + j + 1 positions, and gets zeros when that is none. Rows from
- * row_start[B] to N are left as they were. table [B][max_pages] as in K3dPages. Scores,
+ * first kv_len[b] - rows + j + 1 positions, and gets zeros when that is none. A query row with a
+ * NaN or an infinity, or one that sees a cached row of NaN, gets NaN. Rows from row_start[B] to N
+ * are left as they were. table [B][max_pages] as in K3dPages. Scores,
  * softmax and sums are fp32. Rounded to fp16 are, whatever the types of q and out: q in units of
  * its row (2^-11 of an fp32 value; exact for bf16 within 2^-29 of the row's largest), the softmax
  * weights (2^-11), and rotated keys below 2^-16 of rows with -16 <= e < -2, to multiples of 2^-26

@@ -533,10 +533,13 @@ __device__ __forceinline__ void load_q_rows(const Args &a, const Seg &s, uint32_
                 m = fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
             }
             m = warp_max(m);
-            // m < 2^e; a row with an infinity or a NaN stays as it is
-            const int e = m <= 3.4028234e38f ? max((int)(__float_as_uint(m) >> 23) - 126, -110) : 0;
+            // m < 2^e. A row with an infinity is NaN throughout, as one with a NaN makes its scores: scores
+            // of minus infinity alone would read as positions that are not seen
+            const bool finite = m <= 3.4028234e38f;
+            const int e = finite ? max((int)(__float_as_uint(m) >> 23) - 126, -110) : 0;
             // the sign of the scale goes into q, so that a larger product is a larger score
-            const float up = copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale);
+            const float up = finite ? copysignf(__uint_as_float((uint32_t)(127 + 14 - e) << 23), a.scale)
+                                    : __int_as_float(0x7fc00000);
 #pragma unroll
             for (int c = 0; c < 3; c++) {
                 const int ch = lane + 32 * c;

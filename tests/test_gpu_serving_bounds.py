@@ -83,6 +83,32 @@ def test_attend_small_rotated_keys_under_large_latents(k3, H):
     held(B, B.call(q, H, 3, BF16, F32, 1.0), q, 1.0, F32, False)
 
 
+@pytest.mark.parametrize("qt", [BF16, F32])
+@pytest.mark.parametrize("H", [16, 64])
+def test_attend_queries_with_nan_and_infinity_are_nan(k3, H, qt):
+    """They are NaN wherever they see a position, a single one too, whichever sign the products have, and
+    in items that several CTAs share; the other rows are as without them."""
+    kv, rope = 256, 32
+    reqs = [(1, 1), (1, 1), (2, 1), (130, 2), (3000, 1), (1, 2)]
+    B, g = grid_batch(k3, kv, rope, 64, reqs, 17)
+    N = int(B.start[-1])
+    q = ab.grid_queries(g, N, H, kv, rope, 1.0)
+    clean = B.call(q, H, N, qt, F32, 2.0 ** -6)
+    held(B, clean, q, 2.0 ** -6, F32, True)
+    bad = np.zeros((N, H), bool)
+    for n in range(N):
+        for h, v in ((1, np.inf), (2, -np.inf), (5, np.nan), (7, np.inf)):
+            q[n, h] = np.abs(q[n, h]) if h == 7 else q[n, h]
+            q[n, h, (37 * n + 11 * h) % (kv + rope)] = v
+            bad[n, h] = True
+    q[:, 9], bad[:, 9] = -np.inf, True
+    got = B.call(q, H, N, qt, F32, 2.0 ** -6)
+    none = N - 2                                   # the last request's first row sees nothing
+    assert (got[none] == 0).all()
+    bad[none] = False
+    assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], clean[~bad])
+
+
 class Bf16Loop(Loop):
     """The serving step with bf16 queries, which the kernel takes as they are."""
 
