@@ -1188,7 +1188,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attend4(const __grid_constant__
 // threads that lie beside each other on an SM.
 constexpr int kMergeMax = 512;            // threads
 constexpr int kFew = 8;                   // pieces of an item whose weights are held for all rows
-constexpr int kMaxGrid = 512;             // CTAs of k_attend4 (one per SM)
+constexpr int kMaxGrid = 148;             // CTAs of k_attend4 (one per SM of a B200)
+static_assert(kMaxGrid <= 256, "a thread of the merge for each");
+static_assert((kMaxGrid + 1) * 4 >= kFew * kR, "the weights of a few pieces lie in a piece's four each");
 
 // a piece that saw nothing has no weight
 __device__ __forceinline__ float weigh(float x, float top, float sum)
@@ -1279,43 +1281,32 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 4 : 2) k_attend4_
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
     if (tid == 0) s_c = -1;
-    for (int i = tid; i < grid; i += blockDim.x) {
-        const int4 x = a.info[2 * i], y = a.info[2 * i + 1];
-        s_u0[i] = x.x;
-        s_begin[i] = x.y;
-        s_end[i] = x.z;
-        s_rows[i] = make_int2(y.x, y.y);
-        if (SPLIT && i == 0) s_m = x.w;
+    if (tid < grid) {
+        const int4 x = a.info[2 * tid], y = a.info[2 * tid + 1];
+        s_u0[tid] = x.x;
+        s_begin[tid] = x.y;
+        s_end[tid] = x.z;
+        s_rows[tid] = make_int2(y.x, y.y);
+        if (SPLIT && tid == 0) s_m = x.w;
     }
     __syncthreads();
     // items of fewer rows: m of them share the blocks that one of 64 rows has
     const int sh = SPLIT ? s_m : 0, m = 1 << sh, part = blockIdx.y & (m - 1), which = (blockIdx.x << sh) + part;
     const int y0 = blockIdx.y >> sh, ny = (gridDim.y - part + m - 1) >> sh;
-    int before = 0;
-    for (int i0 = 0; i0 < grid; i0 += blockDim.x) {    // once, but for cards of more SMs than threads
-        const int i = i0 + tid;
-        const bool leads = i >= 1 && i < grid && s_begin[i] >= 0 && s_begin[i] < s_u0[i] && s_u0[i - 1] <= s_begin[i];
-        const unsigned m32 = __ballot_sync(0xffffffffu, leads);
-        if (lane == 0) s_cnt[warp] = __popc(m32);
-        __syncthreads();
-        int rank = before + __popc(m32 & ((1u << lane) - 1u));
-        for (int k = 0; k < nw; k++) {
-            if (k < warp) rank += s_cnt[k];
-            before += s_cnt[k];
-        }
-        if (leads && rank == which) s_c = i;
-        __syncthreads();
-    }
+    const bool leads = tid >= 1 && tid < grid && s_begin[tid] >= 0 && s_begin[tid] < s_u0[tid] && s_u0[tid - 1] <= s_begin[tid];
+    const unsigned m32 = __ballot_sync(0xffffffffu, leads);
+    if (lane == 0) s_cnt[warp] = __popc(m32);
+    __syncthreads();
+    int rank = __popc(m32 & ((1u << lane) - 1u));
+    for (int k = 0; k < warp; k++) rank += s_cnt[k];
+    if (leads && rank == which) s_c = tid;
+    __syncthreads();
     const int c = s_c;
     if (c < 0) return;
     // pieces: CTA c - 1 (its second slot unless the item begins its range), then c, c + 1, ...
     const int2 rw = s_rows[c];
     const int end = s_end[c];
-    int np = 1;
-    for (int i0 = 0; i0 < grid; i0 += blockDim.x) {
-        const int i = i0 + tid;
-        np += __syncthreads_count(i >= c && i < grid && s_u0[i] < end);
-    }
+    const int np = 1 + __syncthreads_count(tid >= c && tid < grid && s_u0[tid] < end);
     const size_t first = (size_t)(c - 1) * 2 + (s_u0[c - 1] == s_begin[c] ? 0 : 1);
     auto slot = [&](int k) { return k == 0 ? first : (size_t)(c - 1 + k) * 2; };
     const float NEG = __int_as_float(0xff800000);
@@ -1415,11 +1406,7 @@ __global__ void __launch_bounds__(FEW ? 256 : kMergeMax, FEW ? 4 : 2) k_attend4_
     }
 }
 
-static int grid_size()
-{
-    const int n = sm_count() > 0 ? sm_count() : 148;
-    return n < kMaxGrid ? n : kMaxGrid;
-}
+static int grid_size() { return sm_count() < kMaxGrid ? sm_count() : kMaxGrid; }
 
 static Split split(int H, int rows) { return {rows, H <= rows ? rows / H : 1, (H + rows - 1) / rows}; }
 
@@ -1431,9 +1418,10 @@ struct Ws {
     size_t part, ml, info, total;
 };
 
+// For the whole of kMaxGrid, so that the size does not depend on when it is asked for.
 static Ws ws_layout(int kv)
 {
-    const size_t g = grid_size();
+    const size_t g = kMaxGrid;
     Ws w;
     w.part = 0;
     w.ml = al256(g * 2 * kR * kv * sizeof(float));

@@ -838,3 +838,20 @@ def test_attend_of_few_rows_beside_other_work(k3, kv, rope, H):
         check(k3.k3d_set_stream(own))
         rt.cudaStreamDestroy(s)
     assert np.array_equal(O.download(np.float32, want.shape), want)
+
+
+def test_attend_workspace_asked_for_before_the_device(k3):
+    """A program may size its buffers before its first library call: the size is the same then, and
+    attention takes it."""
+    import os
+    import subprocess
+    import sys
+    code = ("import k3cuda; lib = k3cuda.load(); c = k3cuda.K3dCache4(512, 64, 64, 9)\n"
+            "a = [lib.k3d_mla_attend4_ws_bytes(c, 3, 5, h) for h in (1, 64, 128)]\n"
+            "k3cuda.check(lib.k3d_init(0))\n"
+            "assert a == [lib.k3d_mla_attend4_ws_bytes(c, 3, 5, h) for h in (1, 64, 128)], a\nprint(*a)")
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(k3cuda.__file__))
+    out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    c = k3cuda.K3dCache4(512, 64, 64, 9)
+    assert [int(v) for v in out.stdout.split()] == [k3.k3d_mla_attend4_ws_bytes(c, 3, 5, h) for h in (1, 64, 128)]
