@@ -408,6 +408,50 @@ def test_plan_taking_and_giving_back_is_the_identity(k3):
     assert all(np.array_equal(a, b) for a, b in zip(before, after))
 
 
+@pytest.mark.parametrize("N", [1024, 1025, 2047, 2048, 2049])
+@pytest.mark.parametrize("B", [64, 256, 257, 1500])
+def test_plan_around_its_row_limits(k3, B, N):
+    """Rows written by the planning CTA (of 256 threads up to 256 requests and 1024 rows, else of 1024) and
+    by the second launch above 2048; several requests to a thread; steps that fill N to the last row."""
+    g = np.random.default_rng(B + N)
+    page, max_pages = 16, 12
+    n_pages = B * 6 + 40
+    free = g.permutation(n_pages).tolist()
+    dev, host = DevPages(k3, page, n_pages, max_pages, B, free), ref.Pages(page, n_pages, max_pages, B, free)
+    lens = np.zeros(B, int)
+    for step in range(4):
+        top = max(1, N // B)
+        new = g.integers(0, min(top, 31) + 1, B)
+        if step == 2:                                              # exactly N rows
+            new[:] = N // B
+            new[:N - new.sum()] += 1
+        assert new.sum() <= N
+        got, want = dev.plan(lens, new, N), host.plan(lens.tolist(), new.tolist(), N)
+        assert want[0] == 0 and got == want, step
+        same_pages(dev, host)
+        lens = np.where(g.random(B) < 0.2, 0, lens + g.integers(0, new + 1))
+
+
+@pytest.mark.parametrize("off", [(1, 1), (0, 2), (3, 0)])
+@pytest.mark.parametrize("N", [2051, 5000])
+def test_plan_rows_at_any_alignment(k3, N, off):
+    """pos and slots need no more than an int's alignment; nothing is written outside them."""
+    g = np.random.default_rng(N)
+    B, page = 50, 16
+    free = g.permutation(700).tolist()
+    dev, host = DevPages(k3, page, 700, 40, B, free), ref.Pages(page, 700, 40, B, free)
+    lens, new = np.zeros(B, int), g.integers(0, N // B + 1, B)
+    L, W = i32(lens), i32(new)
+    rs, kl, st = i32(np.zeros(B + 1)), i32(np.zeros(B)), i32([9])
+    pos, slots = (i32(np.full(N + 8, 77)) for _ in range(2))
+    check(k3.k3d_page_plan(dev.p, L.ptr, W.ptr, B, N, rs.ptr, kl.ptr, pos.ptr + 4 * off[0], slots.ptr + 4 * off[1], st.ptr))
+    check(k3.k3d_sync())
+    want = host.plan(lens.tolist(), new.tolist(), N)
+    for buf, o, w in ((pos, off[0], want[3]), (slots, off[1], want[4])):
+        v = buf.download(np.int32, N + 8)
+        assert v[o:o + N].tolist() == w and (v[:o] == 77).all() and (v[o + N:] == 77).all()
+
+
 @pytest.mark.parametrize("lens,new,N,code", [
     ([10, 20], [200, 200], 1000, k3cuda.K3D_PLAN_PAGES), ([10, 20], [8, 8], 15, k3cuda.K3D_PLAN_ROWS),
     ([10, 20], [1, 400], 1000, k3cuda.K3D_PLAN_TABLE), ([-1, 20], [8, 8], 100, k3cuda.K3D_PLAN_BAD),
@@ -504,6 +548,15 @@ def test_softmax_at_the_ends_of_the_temperatures(k3):
     got = softmax(k3, x, temp)
     softmax_close(got, x, temp)
     assert (got[:3, 3] == 0.5).all() and (got[:3, 4001] == 0.5).all()
+
+
+@pytest.mark.parametrize("rows,V", [(4, 70000), (2, 65537), (1, 300000)])
+def test_softmax_sixteen_ctas_to_a_row(k3, rows, V):
+    """Up to four rows of 65536 and more, greedy rows among them."""
+    g = np.random.default_rng(V)
+    x = (g.standard_normal((rows, V)) * 4).astype(np.float32)
+    temp = np.where(np.arange(rows) % 2 == 1, 0.0, 0.7).astype(np.float32)
+    softmax_close(softmax(k3, x, temp), x, temp)
 
 
 @pytest.mark.parametrize("V", [9000, 9001])
