@@ -14,9 +14,14 @@ most  sum p_t expm1(d_t) |v_t - o| / sum p_t e^(-d_t).  d_t, in natural units:
     rounds by at most 2^-25 of that unit where e < -2: scale sum_rope |q| 2^(-27 + res).
 q is fp16 in units of its row (exact for bf16 within 2^-29 of its largest); the definition is given it so.
 Then, of sum p_t |v_t|: 2^-11 for the fp16 weights, n 2^-22 for the fp32 sums over n positions (weights
-and values, a step each) and 2^-20 for exp2 and the merge. A weight below 2^-14 / 2^7 of the running
-maximum rounds to a multiple of 2^-24 instead: 2^-32 sum |v| 2^(e* - e) (e* the unit of the position with
-the largest s + e, in powers of two). And half a step of the result's type."""
+and values, a step each) and 2^-20 for exp2 and the merge. And half a step of the result's type.
+
+Weights below 2^-14 / 2^7 of the running maximum: the kernel rounds P_t = 2^(a_t - m + 7), a_t = s_t log2(e) +
+r_t, r_t the position's residual exponent, to fp16, whose steps stop at 2^-24, so P_t is off by up to 2^-25
+however small it is. The result is sum P_t (v_t 2^-r_t) / L with L = sum 2^(a_t - r_t - m + 7). m is never
+above the largest a, which position * has, so its term alone gives L >= 2^(7 - r_*): the result moves by at
+most 2^-25 sum |v_t| 2^-r_t / 2^(7 - r_*) = 2^-32 sum |v_t| 2^(r_* - r_t). (In a column where the
+positions of weight hold zeros that is all there is.)"""
 import numpy as np
 
 import serving_ref as ref
@@ -56,8 +61,8 @@ def bound(q, v, exps, kv, scale, n, out="f32", exact=False):
         t = np.einsum("ht,htk->hk", p * np.expm1(d), np.abs(w[None, :, :kv] - o[:, None]))
         t /= (p * np.exp(-d)).sum(1)[:, None]
         t += (2.0 ** -11 + seen * 2.0 ** -22 + 2.0 ** -20) * (p @ np.abs(w[:, :kv]))
-        top = e[(s * np.log2(np.e) + e).argmax(1)]
-        t += 2.0 ** -32 * np.exp2(1.0 * top[:, None]) * (np.abs(w[:, :kv]) * np.exp2(-1.0 * e[:, None])).sum(0)
+        top = res[(s * np.log2(np.e) + res).argmax(1)]
+        t += 2.0 ** -32 * np.exp2(1.0 * top[:, None]) * (np.abs(w[:, :kv]) * np.exp2(-1.0 * res[:, None])).sum(0)
         want[j], tol[j] = o, t + EPS[out] * (np.abs(o) + t)
     return want, tol
 

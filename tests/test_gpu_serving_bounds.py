@@ -109,6 +109,27 @@ def test_attend_queries_with_nan_and_infinity_are_nan(k3, H, qt):
     assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("H", [8, 64])
+def test_attend_columns_of_small_weights_alone(k3, H):
+    """The last position has nearly all the weight and zeros in half of its columns, where what is left are
+    weights of 2^-20 to 2^-34, which fp16 holds to 2^-32."""
+    kv, rope = 128, 16
+    g = np.random.default_rng(19)
+
+    def edit(b, x):
+        x[:] = ab.grid_rows(g, len(x), kv, rope)
+        x[:, kv:] = 0
+        x[:, kv] = -14 - np.arange(len(x)) / 2.0
+        x[-1, kv] = 0
+        x[-1, :kv:2] = 0
+    B = Batch(k3, kv, rope, 16, [(20, 1)], seed=19, edit=edit)
+    q = np.zeros((1, H, kv + rope), np.float32)
+    q[:, :, kv] = 1.0
+    got = B.call(q, H, 1, BF16, F32, 1.0)
+    held(B, got, q, 1.0, F32, True)
+    assert (got[0, :, :kv:2] != 0).any()
+
+
 class Bf16Loop(Loop):
     """The serving step with bf16 queries, which the kernel takes as they are."""
 
