@@ -504,7 +504,8 @@ int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtyp
 /* Absorbed MLA attention over the paged 4-bit cache (the attention step of k3d_mla_decode,
  * following k3_mla_cached, k3_ops.c:321-410): q [N][H][kv_lora + qk_rope] are the absorbed
  * queries of the new rows, out [N][H][kv_lora] the attended latents, each fp32 or bf16 and
- * 16-byte aligned. Request b owns the rows row_start[b] .. row_start[b + 1] and kv_len[b]
+ * 16-byte aligned. (k3d_mla_decode makes the one and consumes the other inside its own call;
+ * here the projections around the attention are the caller's.) Request b owns the rows row_start[b] .. row_start[b + 1] and kv_len[b]
  * cached positions, its new ones (stored before this call) among them; its row j sees the
  * first kv_len[b] - rows + j + 1 positions, and gets zeros when that is none. A query row with a
  * NaN or an infinity, or one that sees a cached row of NaN, gets NaN. Rows from row_start[B] to N
@@ -514,20 +515,22 @@ int    k3d_cache4_load(const K3dCache4 *c, const void *pool, void *out, int dtyp
  * weights (2^-11), and rotated keys below 2^-16 of rows with -16 <= e < -2, to multiples of 2^-26
  * (with e below -16: keys below 2^e, to multiples of 2^(e - 10)). A page id outside the pool, a
  * kv_len above max_pages * page, or a row_start that is not a prefix sum within N raises
- * K3D_EBOUND; such positions count as not there. A call whose tiles of 64 positions, counted for
- * every 64 rows, pass 2^30 raises it too and writes nothing. Weights below about 2^-31 of a row's
- * largest count as 0. N H and max_pages * page are at most 2^30. The workspace belongs to the call
+ * K3D_EBOUND; such positions count as not there. So does a call whose work passes 2^30 units, which
+ * then writes nothing: five and one for each 64 cached positions of its request, for every group of
+ * up to 64 rows (whole tokens of H <= 64 heads, else heads of one token). Weights below about 2^-31
+ * of a row's largest count as 0. N H and max_pages * page are at most 2^30. The workspace belongs to the call
  * until it has run: two calls that may run at the same time (two streams, two graphs) need one
- * each. */
+ * each. Its waits end after about 2 s with K3D_ETIMEOUT, whatever k3d_set_wait_limit says. */
 size_t k3d_mla_attend4_ws_bytes(const K3dCache4 *c, int B, int N, int H);
 int    k3d_mla_attend4(void *out, int out_dtype, const void *q, int q_dtype, const K3dCache4 *c,
                        const void *pool, const int *table, int max_pages, const int *row_start,
                        const int *kv_len, int B, int N, int H, float scale, void *ws,
                        size_t ws_bytes);
 /* p[r] = softmax(logits[r] / temp[r]) over rows of vocab; temp NULL is 1, and a temperature
- * that is not above 0 puts 1 on the first maximum, as k3d_lm_head_argmax picks it. A NaN logit
- * counts as minus infinity; places at +inf share the whole; a row with nothing above minus
- * infinity is zeros. p may be logits itself (in place). */
+ * that is not above 0 puts 1 on the first maximum (-0 and 0 are equal). A NaN logit counts as
+ * minus infinity; places at +inf share the whole; a row with nothing above minus infinity is
+ * zeros. Exponentials are the hardware's fp32 exp2 (two steps), so weights below 2^-126 of the
+ * row's largest are 0. p may be logits itself (in place). */
 int    k3d_logits_softmax(float *p, const float *logits, const float *temp, int rows, int vocab);
 /* Verification of up to K drafted tokens per request (K at most 32; n_draft[b] of them, NULL:
  * K) against the target's probabilities target [B][K + 1][vocab], row i of a request being

@@ -55,10 +55,14 @@
 // 2000, softmax 2300, half of O^T 900) goes round two buffers, which with Q fill the shared
 // memory. The tensor pipe needs 1920 of them (32 for an MMA of S, 48 for one of O^T, both bound
 // by what they read from shared memory), the widening's stores 580. 512 + 64, one call:
-//   64 requests, one token, 16 heads, up to 8192 positions    68 us
-//   16 requests, four tokens, 64 heads, up to 8192 positions  93 us
-//   one request, one token, 64 heads: 1000 positions 17.5 us, 32768 positions 31 us
-// One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge.
+//   64 requests, one token, 16 heads, up to 8192 positions    67 us
+//   16 requests, four tokens, 64 heads, up to 8192 positions  92 us
+//   one request, one token, 64 heads: 1000 positions 16.8 us, 32768 positions 30.5 us
+//   one request, 2048 tokens behind 2048 positions, 64 heads  1.8 ms (486 TFLOP/s)
+// One request is bound by what surrounds its tiles: Q, the first loads, the result, the merge. The
+// constants (units of an item's start, the merge's shares) were measured at 512 + 64 and serve every
+// shape: 128 + 64 takes 44, 57, 14.6 and 22.5 us for the first four. 128 registers: 8 bytes are
+// spilled at 256 and 512 latents, 24 in the merge of few pieces.
 // Measured and left: 18 warps (96 registers, spills), the widening by two groups of four warps
 // that take tiles in turn, pieces of 128 or of 512 latents, two raw buffers ahead (registers
 // again), Q by all 14 warps in one batch (103 -> 121 us), and Q through a bulk copy into the free

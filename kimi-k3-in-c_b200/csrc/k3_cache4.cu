@@ -81,7 +81,7 @@ __device__ __forceinline__ int unit_exp(float a, float m, int le)
 // bits), so no quotient is rounded onto a tie. Traffic (2304 or 1152 bytes in, 417
 // out per row at 512 + 64) and the arithmetic take about as long for prompts, one memory round
 // trip is a decode step's time. 8191 bf16 rows stored and read back as fp32: 14.6 us (ten CTAs an
-// SM; 15.0 without the bound, 17.5 with sixteen, which spill), 64 rows 3.9.
+// SM; 15.0 without the bound, 17.5 with sixteen, which spill), 64 rows 3.8.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kRowWarps, 10) k_cache4_store(Pool4 d, const T *x, size_t ldx,
                                                                 const int *slots, int N)

@@ -278,6 +278,9 @@ extern "C" int k3d_page_plan(const K3dPages *p, const int *len, const int *n_new
     // Up to 2048 rows the one CTA writes them itself; above, a second launch spreads them (us, by
     // the CTA and by a launch: 64 requests of 32 tokens 6.5 and 6.9, of 64 tokens 8.0 and 6.8).
     const int fill = N <= 2048 ? 1 : 0;
+    // A small batch's time is the block's barriers and scans, a large one's the rows to a thread (us
+    // with 256 and 1024 threads: 64 requests of one token 3.2 and 5.5, of four 3.3 and 5.5, 256 of four
+    // 5.8 and 6.0, 64 of 32 tokens 7.8 and 6.7, 1024 of two 10.6 and 7.9; 300 of one token 4.7 and 5.9).
     const int threads = B <= 256 && N <= 1024 ? 256 : 1024;
     launch_pdl(k_page_plan, dim3(1), dim3(threads), 4 * smem, stream(), a, fill);
     note_launch();

@@ -228,8 +228,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_logits_softmax(float *p, cons
 // One cluster per request: each CTA adds its contiguous share of the row, the CTAs' totals
 // meet in distributed shared memory, and the CTA, then the warp, then the quarter of its share
 // that the threshold falls into is walked once more. Bytes: one row of p and one of q per
-// request. 64 registers, and 512 threads while the requests leave SMs idle, else 256: with
-// 512 threads of 100 registers 64 requests took 49 us.
+// request. 64 registers (4 bytes spilled), and 512 threads while all CTAs are resident at once (two
+// to an SM), else 256: with 512 threads of 100 registers, one CTA to an SM, 64 requests took 49 us.
 constexpr int kVMax = 512;                // threads
 constexpr int kVParts = 4;
 constexpr int kMaxDraft = 32;
@@ -443,7 +443,8 @@ __global__ void __launch_bounds__(kVMax, 2) k_spec_verify(Verify a)
 // `many`. Each has 4096 elements at least, and 16384 where the rows fill the card anyway, since a
 // CTA's start and exchanges then cost more than its share (300 rows of 10001: 27 us with a least
 // share of 2048, 12 so; of 40000: 36 and 25; 64 rows of 163840: 24.5 us with eight CTAs, 19.3 with
-// four).
+// four). Verification takes its CTAs by the same rule: 64 requests are 24.2 us with eight and 24.5
+// with four.
 int cluster_of(int rows, int V, int many)
 {
     const long long room = 2LL * sm_count();
@@ -488,8 +489,8 @@ int k3d_logits_softmax(float *p, const float *logits, const float *temp, int row
         return fail(K3D_EINVAL, "k3d_logits_softmax: unaligned pointer");
     if ((long long)rows * 8 > 0x7fffffffLL) return fail(K3D_EINVAL, "k3d_logits_softmax: %d rows", rows);
     K3_TRY(ensure_ctx());
-    // four CTAs to a row where the rows fill the card (320 rows of 163840: 88 us with four, 97
-    // with two, 106 with eight)
+    // four CTAs to a row where the rows fill the card (320 rows of 163840: 81 us with four, 93
+    // with two, 99 with eight)
     const int cs = cluster_of(rows, vocab, 4);
     K3_TRY(wide_clusters(vec4(p) && vec4(logits) && vocab % 4 == 0 ? (const void *)k_logits_softmax<true>
                                                                     : (const void *)k_logits_softmax<false>));
